@@ -276,7 +276,7 @@ def _codes4(cells, at, hs):
     packed = cells[..., at:at + hs // 2]
     u = torch.stack((packed & 15, packed >> 4), -1).flatten(-2).float()
     word = cells[..., at + hs // 2:at + hs // 2 + 4].contiguous().view(torch.int32)
-    return (u - (word & 15).float()) * word.view(torch.float32)
+    return (u - (word & 15).float()) * (word & -16).view(torch.float32)
 
 
 def _keys(case, cells):
@@ -404,7 +404,8 @@ def _exact_rows(case, raw, at):
     rows = torch.empty((raw.shape[0], hs), dtype=torch.float64, device=raw.device)
     rows[:, 0::2] = (raw[:, at:at + hs // 2] % 16).double()
     rows[:, 1::2] = (raw[:, at:at + hs // 2] // 16).double()
-    return (rows - (word % 16).abs().double()) * word.view(torch.float32).double()
+    zp = word % 16  # the word's low four bits; the scale is the word without them
+    return (rows - zp.double()) * (word - zp).view(torch.float32).double()
 
 
 def exact(case, seed):
