@@ -38,6 +38,17 @@ def _sinks_ptr(sinks, nq, mode):
     return sinks.data_ptr()
 
 
+def _lse_ptr(lse_out, rows, nq, mode, out_fp32_lse):
+    """Device pointer of `lse_out` ((tokens, query heads) fp32, base-2 log-sum-exp beside a model-domain output)."""
+    if lse_out is None:
+        return None
+    if mode != 0 or out_fp32_lse is not None:
+        raise ValueError("lse_out goes with the model-domain output (a partial's lse is out_fp32_lse)")
+    if lse_out.dtype != torch.float32 or tuple(lse_out.shape) != (rows, nq) or not lse_out.is_contiguous():
+        raise ValueError(f"lse_out must be contiguous fp32 ({rows}, {nq})")
+    return lse_out.data_ptr()
+
+
 def _dtype_code(t, what):
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -224,7 +235,7 @@ def decode_num_splits(num_seqs, num_kv_heads, max_seqlen_k, sms):
 def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, seqused_k, max_seqlen_k,
                  softmax_scale, block_table, k_scale_cache, v_scale_cache, num_splits=None, q_rotated=False,
                  out_fp32_lse=None, ws=None, partials_only=False, tokens_after_keys=0, sliding_window=0,
-                 softcap=0.0, sinks=None):
+                 softcap=0.0, sinks=None, lse_out=None):
     """Split-KV decode of up to 32 query rows per KV head (4 MTP tokens x 6 heads) over the paged cache.
 
     q / out (tokens, query heads, hs). When `out_fp32_lse` is a tensor (tokens, query heads) fp32, `out` must be fp32
@@ -235,7 +246,9 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
     key k iff k <= seqused_k - qlen + i + tokens_after_keys. sliding_window: vLLM's SLIDING_WINDOW (1 +
     window_size[0], 0 = none): that token then sees only the keys k > its last key - sliding_window. softcap > 0:
     vLLM's logit softcap, every score S becomes softcap * tanh(S / softcap). sinks: None or (query heads,) sink
-    logits whose exp joins every row's softmax denominator (vLLM's attention sinks; model-domain output only)."""
+    logits whose exp joins every row's softmax denominator (vLLM's attention sinks; model-domain output only).
+    lse_out: None or (tokens, query heads) fp32, filled with the base-2 log-sum-exp of each row's scaled scores, sinks
+    included (what `accumulate_attention_weights` takes), beside a model-domain output."""
     hs = q.shape[-1]
     nq = q.shape[1]
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
@@ -267,6 +280,7 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
         if out.dtype != q.dtype:
             raise TypeError("out dtype must match q")
         mode, lse_ptr = 0, None
+    lse_ptr = _lse_ptr(lse_out, q.shape[0], nq, mode, out_fp32_lse) or lse_ptr
     _lib.call("qp_paged_decode", lay.fmt, dt, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
               out.stride(1), q.shape[0], num_seqs, cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q),
               block_table.data_ptr(), block_table.stride(0), *lay.args(), nq, nkv, hs, float(softmax_scale),
@@ -318,12 +332,12 @@ def fold_peer_partials(bases, rank, world, epoch, num_tokens, num_heads, head_si
 
 
 def prefill(q, key_cache, value_cache, out, *, block_row, n, softmax_scale, k_scale_cache, v_scale_cache,
-            q_rotated=False, out_fp32_lse=None, ws=None, tokens_after_keys=0):
+            q_rotated=False, out_fp32_lse=None, ws=None, tokens_after_keys=0, lse_out=None):
     """Chunk prefill of one sequence on the tensor cores: q (qlen, query heads, hs) are the last qlen positions of a
     context of n cached tokens (causal among themselves); block_row is the sequence's int32 block-table row.
     `out` gets the model-domain output in q's dtype, or with `out_fp32_lse` the fp32 RHT-domain output and its
     base-2 lse (vllm_quantpack/attention/int4_prefill.py:203-232 returns the RHT-domain output for rotated queries).
-    tokens_after_keys as in paged_decode (n >= qlen - tokens_after_keys)."""
+    tokens_after_keys (n >= qlen - tokens_after_keys) and lse_out as in paged_decode."""
     hs, nq, qlen = q.shape[-1], q.shape[1], q.shape[0]
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
     if block_row.dtype != torch.int32 or block_row.stride(-1) != 1:
@@ -342,6 +356,7 @@ def prefill(q, key_cache, value_cache, out, *, block_row, n, softmax_scale, k_sc
         if out.dtype != q.dtype:
             raise TypeError("out dtype must match q")
         mode, lse_ptr = 0, None
+    lse_ptr = _lse_ptr(lse_out, qlen, nq, mode, out_fp32_lse) or lse_ptr
     _lib.call("qp_prefill", lay.fmt, dt, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
               out.stride(1), qlen, int(n), block_row.data_ptr(), *lay.args(), nq, lay.nkv, hs, float(softmax_scale),
               rht.device_sign_bits(hs, q.device).data_ptr(), int(bool(q_rotated)), int(tokens_after_keys), mode,
@@ -351,13 +366,13 @@ def prefill(q, key_cache, value_cache, out, *, block_row, n, softmax_scale, k_sc
 
 def prefill_varlen(q, key_cache, value_cache, out, *, cu_seqlens_q, seqused_k, max_seqlen_k, block_table,
                    softmax_scale, k_scale_cache, v_scale_cache, q_rotated=False, out_fp32_lse=None, ws=None,
-                   sliding_window=0, softcap=0.0, sinks=None):
+                   sliding_window=0, softcap=0.0, sinks=None, lse_out=None):
     """Several short prefill chunks in ONE launch (the reference's Triton sub-batch of the chunks that are not long,
     vllm_quantpack/attention/int4_kv.py:313-323): request i's query tokens q[cu_seqlens_q[i]:cu_seqlens_q[i + 1]] are
     the last positions of its context of seqused_k[i] cached tokens, causal among themselves, read through
     block_table[i]. Split on the device into sub-sequences of 32 / group tokens for the split-KV kernel, so nothing
     is read back to the host; max_seqlen_k (a host int, an upper bound of seqused_k) sizes the split count.
-    `out` as in prefill; sliding_window, softcap and sinks as in paged_decode."""
+    `out` as in prefill; sliding_window, softcap, sinks and lse_out as in paged_decode."""
     hs, nq, T = q.shape[-1], q.shape[1], q.shape[0]
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
     for name, t in (("cu_seqlens_q", cu_seqlens_q), ("seqused_k", seqused_k), ("block_table", block_table)):
@@ -380,6 +395,7 @@ def prefill_varlen(q, key_cache, value_cache, out, *, cu_seqlens_q, seqused_k, m
         if out.dtype != q.dtype:
             raise TypeError("out dtype must match q")
         mode, lse_ptr = 0, None
+    lse_ptr = _lse_ptr(lse_out, T, nq, mode, out_fp32_lse) or lse_ptr
     _lib.call("qp_prefill_varlen", lay.fmt, dt, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
               out.stride(0), out.stride(1), T, chunks, cu_seqlens_q.data_ptr(), seqused_k.data_ptr(),
               max_k, block_table.data_ptr(), block_table.stride(0), *lay.args(), nq, lay.nkv, hs,

@@ -1,6 +1,6 @@
 // K1: split-KV paged decode over an int4_per_token_head / k8v4_per_token_head cache, up to 32 query rows
 //     (qlen x query heads per KV head) per KV head, head size 256 or 512, on the 5th-generation tensor cores
-//     (tcgen05 + TMEM); K0q: the query preparation it reads; K2: log-sum-exp merge of the segments with the inverse
+//     (tcgen05 + TMEM; head 128 is qp_decode128.cu, behind the same entry points); K0q: the query preparation it reads; K2: log-sum-exp merge of the segments with the inverse
 //     RHT and the attention sinks fused in. At head 512 the same kernel also serves chunk prefill, as decodes of a
 //     few query tokens each over the chunk's causal prefixes (qp_prefill), and at both head sizes the short chunks of
 //     a step in one launch (qp_prefill_varlen). A second instantiation (FEAT) applies vLLM's sliding window and logit
@@ -55,6 +55,7 @@
 
 #include "qp_api_internal.h"
 #include "qp_common.cuh"
+#include "qp_decode.cuh"
 #include "qp_tcgen05.cuh"
 
 namespace qp {
@@ -62,7 +63,6 @@ namespace qp {
 constexpr int DEC_TILE = 128;  // keys per tile (TMEM lanes of the QK accumulator)
 constexpr int P_KGROUP = 128;                    // bytes between the 8-key groups of P^T (LBO of its descriptor)
 constexpr int P_NGROUP = DEC_TILE / 8 * P_KGROUP;  // bytes between its 8-row groups (SBO)
-constexpr int DEC_MAX_ROWS = 32;
 #ifndef QP_DEC_SMX_HALVES
 #define QP_DEC_SMX_HALVES 1
 #endif
@@ -90,52 +90,7 @@ struct DecWarps {
 };
 // prepared query row: HS fp16 in operand order, then 4 fp32 (row scale, three zero words)
 constexpr int q_rec_bytes(int hs) { return hs * 2 + 16; }
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float RESCALE_SLACK = 8.f;
 constexpr int BAR_SMX = 1;  // named barrier of the softmax warps
-
-struct DecodeParams {
-  const void* q;
-  int64_t q_st, q_sh;  // element strides of q (token, head)
-  const int32_t* cu_seqlens_q;
-  const int32_t* seqused_k;
-  const int32_t* block_table;
-  int64_t bt_stride;
-  const uint8_t* cache;
-  int block_size;
-  int64_t block_stride, head_stride;  // bytes; cells of one (block, head) are contiguous (slot stride == cell)
-  int nq, nkv, group;  // query heads, KV heads, query heads per KV head
-  float qk_scale;      // softmax_scale / head_size * log2(e)
-  const uint32_t* sign_bits;
-  int q_rotated;        // q already in the RHT domain
-  const uint8_t* qrec;  // prepared query rows: [kv head][token][query head of the group] x q_rec_bytes(HS)
-  int64_t num_tokens;
-  int tokens_after;  // sequence tokens after this call's keys (held by other ranks), clamped to the query tokens
-  // chunk_q > 0: the num_tokens query tokens are ONE sequence's chunk (its last positions, causal among themselves)
-  // over chunk_n cached keys through block-table row 0, served as sub-sequences of chunk_q tokens (grid z), each
-  // reading only the keys its last token sees. cu_seqlens_q / seqused_k are not read.
-  int chunk_q, chunk_n;
-  // subseq != null: sequence z of the grid is subseq[z] = {first query token, query tokens, keys its last token
-  // sees, block-table row}, causal inside it (built on the device by varlen_table_kernel; entries past the real ones
-  // hold 0 query tokens). cu_seqlens_q / seqused_k are not read.
-  const int4* subseq;
-  // window > 0: vLLM's SLIDING_WINDOW (1 + window_size[0]): a query token whose last visible key is p sees the keys
-  // [p - window + 1, p] only (vllm/v1/attention/ops/triton_attention_helpers.py:196-218, vLLM 0.22)
-  int window;
-  // softcap > 0: every score S (natural units) becomes softcap x tanh(S / softcap) before the softmax, vLLM's
-  // apply_softcap (vllm/v1/attention/ops/triton_attention_helpers.py:28-36, triton_unified_attention.py:513-514)
-  float softcap;
-  int num_splits;
-  float* part_o;    // [tokens][nq][splits][HS]
-  float* part_lse;  // [tokens][nq][splits], log2 units
-};
-
-template <int FMT, int HS>
-struct Cell {
-  static constexpr int KB = FMT == FMT_INT4 ? HS / 2 : HS;  // key bytes
-  static constexpr int BYTES = KB + 8 + HS / 2;
-  static constexpr int KS = KB, V = KB + 4, VS = KB + 4 + HS / 2;  // field offsets
-};
 
 // TMEM columns (512) of the head size's operands and accumulators.
 //   HS 256: key operand chunks at [0, 128) and [384, 512); two 64-key value slots (two channel tiles of 32 columns)
@@ -253,24 +208,6 @@ __device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const float (&v)[NR
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// capl x tanh(t / capl) for a score t in log2 units (capl = softcap x log2 e, cap_k = 2 log2 e / capl), from
-// tanh(y) = 1 - 2 / (e^{2y} + 1) taken on |y| and given t's sign: absolute error ~1e-7 x capl, which is what a softmax
-// argument needs (no cancellation matters once it is multiplied back by capl); e^{2|y|} = 2^{|t| cap_k}, its exponent
-// held below 64 so the quotient stays finite.
-__device__ __forceinline__ float softcap_log2(float t, float capl, float cap_k) {
-  const float a = fast_exp2(fminf(fabsf(t) * cap_k, 64.f));
-  return copysignf(capl * (1.f - __fdividef(2.f, a + 1.f)), t);
-}
-
-// k index (0..HS-1) of the QK operand that carries channel c. int4: column j = 4 w + m of a key's TMEM lane holds
-// the pair lop3'd from word w (shifted right 8 for m >= 2; low nibbles for even m, high for odd), i.e. channels
-// 8 w + m (low half) and 8 w + m + 4 (high half); k8v4: the natural order (prmt takes bytes 0, 1 then 2, 3).
-template <int FMT>
-__host__ __device__ __forceinline__ int qk_k_of_channel(int c) {
-  if constexpr (FMT == FMT_INT4) return 8 * (c >> 3) + 2 * (c & 3) + ((c >> 2) & 1);
-  else return c;
-}
-
 // ---------------------------------------------------------------------------------------------------- K0q
 // One warp per (query token, query head): the row as K1 reads it (q_rec_bytes(HS)): HS fp16 in the k order of the
 // QK operand, scaled by a power of two (|q| < 2^14; int4: the high-nibble channels by a further 2^-4); then the
@@ -359,30 +296,9 @@ __global__ void __maxnreg__((DecWarps<HS, RL>::REGS)) decode_kernel(const Decode
   // grid's completion before reading anything.
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // the sequence's query tokens [q0, q0 + qlen), its keys [0, n), the last key its first token sees (before clamping
-  // to n - 1) and its block-table row
-  int q0, qlen, n, vis_base;
-  const int32_t* btab;
-  if (p.subseq != nullptr) {
-    const int4 e = p.subseq[seq];
-    q0 = e.x;
-    qlen = e.y;
-    n = e.z;
-    vis_base = n - qlen;
-    btab = p.block_table + static_cast<int64_t>(e.w) * p.bt_stride;
-  } else if (p.chunk_q > 0) {
-    q0 = seq * p.chunk_q;
-    qlen = min(p.chunk_q, static_cast<int>(p.num_tokens) - q0);
-    vis_base = p.chunk_n - static_cast<int>(p.num_tokens) + q0 + p.tokens_after;
-    n = min(p.chunk_n, vis_base + qlen);
-    btab = p.block_table;
-  } else {
-    q0 = p.cu_seqlens_q[seq];
-    qlen = p.cu_seqlens_q[seq + 1] - q0;
-    n = p.seqused_k[seq];
-    vis_base = n - qlen + p.tokens_after;
-    btab = p.block_table + static_cast<int64_t>(seq) * p.bt_stride;
-  }
+  const DecodeSpan span = decode_span(p, seq);
+  const int q0 = span.q0, qlen = span.qlen, n = span.n, vis_base = span.vis_base;
+  const int32_t* btab = span.btab;
   const int rows = qlen * p.group;
   if (qlen <= 0) return;
   // with a sliding window the splits share the tiles from the one holding the first token's first key: the later
@@ -1093,7 +1009,7 @@ struct MergeParams {
   int mode;  // 0: inverse RHT / head, cast to the model dtype; 1: fp32 RHT-domain O and lse (log2) out
   void* out;
   int64_t out_st, out_sh;  // element strides of out
-  float* lse_out;          // mode 1 (may be null)
+  float* lse_out;          // base 2, the sinks included (may be null)
   int64_t lo_t, lo_h;
   const uint32_t* sign_bits;
   float out_scale;  // multiplies the output (mode 0: 1 / head)
@@ -1169,6 +1085,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeParams 
   __syncthreads();
   const float T = tot_sm;
   const float inv = T > 0.f ? 1.f / T : 0.f;
+  if (tid == 0 && p.lse_out) p.lse_out[tok * p.lo_t + qh * p.lo_h] = T > 0.f ? M + log2f(T) : -INFINITY;
   if (p.mode == 1) {
     for (int c = tid; c < HS; c += MERGE_THREADS) {
       float v = 0.f;
@@ -1176,7 +1093,6 @@ __global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeParams 
       for (int s = 0; s < SG; ++s) v += acc_sm[s][c];
       reinterpret_cast<float*>(p.out)[tok * p.out_st + qh * p.out_sh + c] = v * inv;
     }
-    if (tid == 0 && p.lse_out) p.lse_out[tok * p.lo_t + qh * p.lo_h] = T > 0.f ? M + log2f(T) : -INFINITY;
     return;
   }
   if (tid < 32) {
@@ -1295,6 +1211,7 @@ static int launch_decode_fmt(int dtype, int hs, const DecodeParams& dp, int rows
 }
 
 static int launch_decode(int fmt, int dtype, int hs, const DecodeParams& dp, int rows, int grid_z, cudaStream_t st) {
+  if (hs == 128) return launch_decode128(fmt, dtype, dp, rows, grid_z, st);
   return fmt == FMT_INT4 ? launch_decode_fmt<FMT_INT4>(dtype, hs, dp, rows, grid_z, st)
                          : launch_decode_fmt<FMT_K8V4>(dtype, hs, dp, rows, grid_z, st);
 }
@@ -1342,8 +1259,8 @@ static int decode_check_cache(const char* who, int fmt, int dtype, int head_size
                               int64_t ks_off, int64_t v_off, int64_t vs_off) {
   if (fmt != FMT_INT4 && fmt != FMT_K8V4) return set_error(QP_ERR_UNSUPPORTED, "%s: format %d", who, fmt);
   if (dtype != DT_BF16 && dtype != DT_F16) return set_error(QP_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
-  if (head_size != 256 && head_size != 512)
-    return set_error(QP_ERR_UNSUPPORTED, "%s: head size %d (this build: 256, 512)", who, head_size);
+  if (head_size != 128 && head_size != 256 && head_size != 512)
+    return set_error(QP_ERR_UNSUPPORTED, "%s: head size %d (this build: 128, 256, 512)", who, head_size);
   const int kb = fmt == FMT_INT4 ? head_size / 2 : head_size;
   const int cell = kb + 8 + head_size / 2;
   if (slot_stride != cell)

@@ -960,7 +960,7 @@ static int64_t prefill_ws_bytes(int qlen, int nq, int64_t nt, int parts) {
 extern "C" int64_t qp_prefill_workspace_bytes(int qlen, int n, int num_q_heads, int num_kv_heads, int head_size,
                                               int tokens_after_keys) {
   if (qlen <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || tokens_after_keys < 0) return 0;
-  if (head_size == 512) return decode_chunk_workspace_bytes(qlen, n, num_q_heads, num_kv_heads, head_size);
+  if (head_size != PF_HS) return decode_chunk_workspace_bytes(qlen, n, num_q_heads, num_kv_heads, head_size);
   const int after = std::min(tokens_after_keys, qlen);
   const int group = num_q_heads / num_kv_heads;
   // either cache format (the chunk count depends on the cell size)
@@ -1034,11 +1034,11 @@ __global__ void __launch_bounds__(32 * FOLD_WARPS) prefill_fold_kernel(const flo
   const float inv = T > 0.f ? 1.f / T : 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= inv;
+  if (lane == 0 && lse_out) lse_out[r] = T > 0.f ? M + log2f(T) : -INFINITY;
   if (mode == 1) {
     float* dst = reinterpret_cast<float*>(out) + tok * out_st + qh * out_sh + 8 * lane;
 #pragma unroll
     for (int i = 0; i < 8; ++i) dst[i] = x[i];
-    if (lane == 0 && lse_out) lse_out[r] = T > 0.f ? M + log2f(T) : -INFINITY;
     return;
   }
   warp_wht<8>(x, lane);
@@ -1066,8 +1066,8 @@ extern "C" int qp_prefill(int fmt, int dtype, const void* q, int64_t q_stride_to
                           float* lse_out, void* workspace, int64_t workspace_bytes, void* stream) {
   if (fmt != FMT_INT4 && fmt != FMT_K8V4) return set_error(QP_ERR_UNSUPPORTED, "prefill: format %d", fmt);
   if (dtype != DT_BF16 && dtype != DT_F16) return set_error(QP_ERR_UNSUPPORTED, "prefill: dtype %d", dtype);
-  if (head_size != PF_HS && head_size != 512)
-    return set_error(QP_ERR_UNSUPPORTED, "prefill: head size %d (this build: 256, 512)", head_size);
+  if (head_size != PF_HS && head_size != 128 && head_size != 512)
+    return set_error(QP_ERR_UNSUPPORTED, "prefill: head size %d (this build: 128, 256, 512)", head_size);
   const int after = std::min(std::max(tokens_after_keys, 0), std::max(qlen, 0));  // >= qlen: nothing masked
   if (tokens_after_keys < 0 || qlen < 0 || n < qlen - after || (qlen > 0 && n <= 0) || num_kv_heads <= 0 ||
       num_q_heads <= 0 || num_q_heads % num_kv_heads)
@@ -1075,7 +1075,8 @@ extern "C" int qp_prefill(int fmt, int dtype, const void* q, int64_t q_stride_to
                      num_kv_heads);
   if (qlen == 0) return QP_OK;
   if (out_mode != 0 && out_mode != 1) return set_error(QP_ERR_INVALID, "prefill: out_mode %d", out_mode);
-  if (head_size == 512) {  // O^T of a 128-query tile would need all of TMEM: the split-KV kernel's chunk mode
+  if (head_size != PF_HS) {  // 512: O^T of a 128-query tile would need all of TMEM; 128 has no such kernel: the
+                             // split-KV kernels' chunk mode
     if (!q || !out || !block_row || !cache || !rht_sign_bits || !workspace)
       return set_error(QP_ERR_INVALID, "prefill: null pointer");
     return decode_chunk_prefill(fmt, dtype, q, q_stride_token, q_stride_head, out, out_stride_token, out_stride_head,
