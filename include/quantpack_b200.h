@@ -86,6 +86,12 @@ int qp_single_rht(const float* x, float* y, int64_t rows, int head_size, int inv
  * `segments_for` / `decode_tiles` (vllm_quantpack/attention/int4_kv.py:66-78). */
 int qp_decode_num_splits(int num_seqs, int num_kv_heads, int max_seqlen_k, int sm_count);
 
+/* The same for a head size: 256 and 512 as above; at 128 the most partials a row of a batch gets, where max_rows is
+ * max_seqlen_q * (num_q_heads / num_kv_heads) (the batch's tiles are shared evenly over the GPU whatever the lengths,
+ * and num_splits bounds the shares that meet in one sequence and KV head). */
+int qp_decode_num_splits_head(int head_size, int max_rows, int num_seqs, int num_kv_heads, int max_seqlen_k,
+                              int sm_count);
+
 /* Bytes of workspace qp_paged_decode needs (the split-KV partials). Stands in for the segment buffers vLLM's
  * metadata builder allocates (vllm_quantpack/attention/int4_kv.py:229-257). */
 int64_t qp_decode_workspace_bytes(int64_t num_q_tokens, int num_q_heads, int head_size, int num_splits);

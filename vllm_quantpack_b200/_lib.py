@@ -25,6 +25,7 @@ SIGNATURES = {
                                        _P, _I, _P]),
     "qp_single_rht": (_I, [_P, _P, _L, _I, _I, _P, _P]),
     "qp_decode_num_splits": (_I, [_I, _I, _I, _I]),
+    "qp_decode_num_splits_head": (_I, [_I, _I, _I, _I, _I, _I]),
     "qp_decode_workspace_bytes": (_L, [_L, _I, _I, _I]),
     "qp_paged_decode": (_I, [_I, _I, _P, _L, _L, _P, _L, _L, _L, _I, _P, _P, _I, _P, _L, _P, _I, _L, _L, _L, _L, _L,
                              _L, _L, _I, _I, _I, _F, _P, _I, _I, _I, _F, _P, _I, _P, _I, _P, _L, _P]),

@@ -255,8 +255,12 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
     nkv = lay.nkv
     num_seqs = cu_seqlens_q.shape[0] - 1
     if num_splits is None:
-        num_splits = decode_num_splits(num_seqs, nkv, window_keys(max_seqlen_k, sliding_window, max_seqlen_q),
-                                       sm_count(q.device))
+        keys = window_keys(max_seqlen_k, sliding_window, max_seqlen_q)
+        if hs == 128:
+            num_splits = _memo("qp_decode_num_splits_head", hs, int(max_seqlen_q) * (nq // nkv), num_seqs, nkv, keys,
+                               sm_count(q.device))
+        else:
+            num_splits = decode_num_splits(num_seqs, nkv, keys, sm_count(q.device))
     wbytes = _memo("qp_decode_workspace_bytes", int(q.shape[0]), int(nq), int(hs), int(num_splits))
     if ws is None:
         ws = workspace(q.device, wbytes)

@@ -999,26 +999,6 @@ __global__ void __maxnreg__((DecWarps<HS, RL>::REGS)) decode_kernel(const Decode
 }
 
 // ---------------------------------------------------------------------------------------------------- K2 merge
-struct MergeParams {
-  const float* part_o;
-  const float* part_lse;     // log2 units
-  int64_t po_t, po_h, po_s;  // element strides of part_o (token, head, part); channel stride 1
-  int64_t pl_t, pl_h, pl_s;
-  int num_splits;
-  int nq;
-  int mode;  // 0: inverse RHT / head, cast to the model dtype; 1: fp32 RHT-domain O and lse (log2) out
-  void* out;
-  int64_t out_st, out_sh;  // element strides of out
-  float* lse_out;          // base 2, the sinks included (may be null)
-  int64_t lo_t, lo_h;
-  const uint32_t* sign_bits;
-  float out_scale;  // multiplies the output (mode 0: 1 / head)
-  // mode 0, may be null: per query head, a sink logit (natural units) whose exp joins every row's softmax
-  // denominator once, vLLM's attention sinks (vllm/v1/attention/ops/triton_attention_helpers.py:108-138: the row
-  // maximum starts at the sink with sum 1 in one segment only; triton_unified_attention.py:356-359)
-  const float* sinks;
-};
-
 constexpr int MERGE_THREADS = 512;
 
 template <int DT, int HS>
@@ -1137,6 +1117,7 @@ static int merge_dispatch(const MergeParams& mp, int dtype, int head_size, int64
   if (mp.num_splits > 1024) return set_error(QP_ERR_UNSUPPORTED, "merge: %d partials > 1024", mp.num_splits);
   if (num_tokens > 0x7fffffff) return set_error(QP_ERR_UNSUPPORTED, "merge: too many tokens");
   const int nt = static_cast<int>(num_tokens);
+  if (head_size == 128 && pdl) return launch_merge128(mp, dtype, nt, st);  // the split kernel's own partials
   switch (head_size) {
     case 256:
       return dtype == DT_BF16 ? launch_merge<DT_BF16, 256>(mp, nt, st, pdl) : launch_merge<DT_F16, 256>(mp, nt, st, pdl);
@@ -1239,6 +1220,12 @@ extern "C" int qp_decode_num_splits(int num_seqs, int num_kv_heads, int max_seql
     }
   }
   return best;
+}
+
+extern "C" int qp_decode_num_splits_head(int head_size, int max_rows, int num_seqs, int num_kv_heads,
+                                         int max_seqlen_k, int sm_count) {
+  if (head_size == 128) return decode128_num_splits(max_rows, num_seqs, num_kv_heads, max_seqlen_k, sm_count);
+  return qp_decode_num_splits(num_seqs, num_kv_heads, max_seqlen_k, sm_count);
 }
 
 // Workspace of qp_paged_decode: [part_o rows x head fp32][part_lse rows fp32, 256-aligned][prepared query rows
@@ -1352,6 +1339,7 @@ extern "C" int qp_paged_decode(int fmt, int dtype, const void* q, int64_t q_stri
   dp.q_sh = q_stride_head;
   dp.cu_seqlens_q = cu_seqlens_q;
   dp.seqused_k = seqused_k;
+  dp.num_seqs = num_seqs;
   dp.block_table = block_table;
   dp.bt_stride = block_table_stride;
   dp.cache = static_cast<const uint8_t*>(cache);

@@ -42,6 +42,9 @@ struct DecodeParams {
   // softcap > 0: every score S (natural units) becomes softcap x tanh(S / softcap) before the softmax, vLLM's
   // apply_softcap (vllm/v1/attention/ops/triton_attention_helpers.py:28-36, triton_unified_attention.py:513-514)
   float softcap;
+  // head 128 only: the num_seqs sequences of cu_seqlens_q / seqused_k share the grid's CTAs evenly whatever their
+  // lengths (set by launch_decode128), instead of num_splits equal parts of each
+  int num_seqs, balanced;
   int num_splits;
   float* part_o;    // [tokens][nq][splits][HS]
   float* part_lse;  // [tokens][nq][splits], log2 units
@@ -104,8 +107,32 @@ __host__ __device__ __forceinline__ int qk_k_of_channel(int c) {
   else return c;
 }
 
-// Launches the head-128 kernel (qp_decode128.cu) on the parameters of launch_decode; `rows` query rows per KV head at
-// most.
-int launch_decode128(int fmt, int dtype, const DecodeParams& dp, int rows, int grid_z, cudaStream_t st);
+// The merge of split partials (K2, and its head-128 form).
+struct MergeParams {
+  const float* part_o;
+  const float* part_lse;     // log2 units
+  int64_t po_t, po_h, po_s;  // element strides of part_o (token, head, part); channel stride 1
+  int64_t pl_t, pl_h, pl_s;
+  int num_splits;
+  int nq;
+  int mode;  // 0: inverse RHT / head, cast to the model dtype; 1: fp32 RHT-domain O and lse (log2) out
+  void* out;
+  int64_t out_st, out_sh;  // element strides of out
+  float* lse_out;          // base 2, the sinks included (may be null)
+  int64_t lo_t, lo_h;
+  const uint32_t* sign_bits;
+  float out_scale;  // multiplies the output (mode 0: 1 / head)
+  // mode 0, may be null: per query head, a sink logit (natural units) whose exp joins every row's softmax
+  // denominator once, vLLM's attention sinks (vllm/v1/attention/ops/triton_attention_helpers.py:108-138: the row
+  // maximum starts at the sink with sum 1 in one segment only; triton_unified_attention.py:356-359)
+  const float* sinks;
+};
+
+// Launches the head-128 kernel (qp_decode128.cu) on the parameters of launch_decode, `rows` query rows per KV head at
+// most, and its merge.
+int launch_decode128(int fmt, int dtype, DecodeParams dp, int rows, int grid_z, cudaStream_t st);
+// Partials a row of a head-128 decode batch may have.
+int decode128_num_splits(int rows, int num_seqs, int num_kv_heads, int max_seqlen_k, int sm_count);
+int launch_merge128(const MergeParams& mp, int dtype, int num_tokens, cudaStream_t st);
 
 }  // namespace qp
