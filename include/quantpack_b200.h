@@ -115,13 +115,14 @@ int64_t qp_decode_workspace_bytes(int64_t num_q_tokens, int num_q_heads, int hea
  * denominator once, as vLLM's attention sinks (triton_attention_helpers.py:108-138: the row maximum starts at the
  * sink with sum 1, in one segment only).
  * out_mode 0: out in dtype, model domain. out_mode 1: out fp32 in the RHT domain and lse_out (tokens, num_q_heads)
- * the base-2 log-sum-exp of the scaled scores (the partial a sequence-parallel rank exchanges). out_mode 2: the
+ * the base-2 log-sum-exp of the scaled scores (the partial a sequence-parallel rank exchanges); with out_mode 0 a
+ * lse_out that is not null gets it too, the sinks included. out_mode 2: the
  * split partials only, left in the workspace as part_o (tokens, num_q_heads, num_splits, head_size) fp32 followed by
  * part_lse (tokens, num_q_heads, num_splits) base-2, for a caller that folds them with qp_merge_attn_partials.
  * Replaces the plugin's split-KV decode: the patched `_launch_packed_attn` (int4_kv.py:98-122, 212-216) with its 3D
  * kernel `_attn_packed_qp` / `_attn_k8v4_qp` (int4_kv.py:80-146) and vLLM's reduce_segments, reached through
  * `unified_attention_int4` (int4_kv.py:294-307). Needs HND cells (slot_stride == cell bytes), block_size % 16 == 0,
- * head_size 256 or 512, a 16-byte aligned cache and qp_decode_workspace_bytes() of workspace. */
+ * head_size 128, 256 or 512, a 16-byte aligned cache and qp_decode_workspace_bytes() of workspace. */
 int qp_paged_decode(int fmt, int dtype, const void* q, int64_t q_stride_token, int64_t q_stride_head, void* out,
                     int64_t out_stride_token, int64_t out_stride_head, int64_t num_q_tokens, int num_seqs,
                     const int32_t* cu_seqlens_q, const int32_t* seqused_k, int max_seqlen_q,
@@ -141,8 +142,8 @@ int64_t qp_prefill_workspace_bytes(int qlen, int n, int num_q_heads, int num_kv_
  * among themselves) attend to the whole cached context through block_row (that sequence's block-table row), on the
  * tcgen05 tensor cores with every key / value tile dequantised in shared memory (no scratch unpack of the cache).
  * out_mode / lse_out / q_rotated / tokens_after_keys as in qp_paged_decode (n >= qlen - tokens_after_keys);
- * head_size 256, or 512 (there the chunk runs on the split-KV decode kernel as decodes of 32 / (query heads per KV
- * head) tokens over its causal prefixes: O of a 128-query tile alone would fill TMEM); HND cells,
+ * head_size 256, or 128 or 512 (there the chunk runs on the split-KV decode kernel as decodes of 32 / (query heads per
+ * KV head) tokens over its causal prefixes: at 512, O of a 128-query tile alone would fill TMEM); HND cells,
  * block_size % 16 == 0.
  * Replaces vllm_quantpack/attention/int4_prefill.py:203-232 `prefill_sequence` (16k-token bf16 unpacks +
  * FlashAttention 2 + log-sum-exp fold) and the Triton 2D path of int4_kv.py:113-119, reached through
@@ -165,7 +166,7 @@ int64_t qp_prefill_varlen_workspace_bytes(int64_t num_q_tokens, int num_chunks, 
  * the call never reads back to the host. max_seqlen_k bounds the keys any query token sees (seqused_k, or with a
  * sliding window min(seqused_k, sliding_window + 158)); it sizes the split count and the workspace. The chunks run
  * on the split-KV decode kernel as sub-sequences of 32 / (query heads per KV head) tokens. out / out_mode / lse_out /
- * q_rotated / sliding_window / softcap / sinks as in qp_paged_decode (out_mode 0 or 1); head_size 256 or 512; HND cells,
+ * q_rotated / sliding_window / softcap / sinks as in qp_paged_decode (out_mode 0 or 1); head_size 128, 256 or 512; HND cells,
  * block_size % 16 == 0.
  * Replaces the Triton 2D sub-batch that the plugin runs for every chunk that is not long (int4_kv.py:113-119,
  * 313-323). */
@@ -230,6 +231,54 @@ int qp_merge_attn_partials(int dtype, int head_size, int64_t num_tokens, int num
                            int64_t pl_stride_head, int64_t pl_stride_part, int out_mode, void* out,
                            int64_t out_stride_token, int64_t out_stride_head, float* lse_out,
                            const uint32_t* rht_sign_bits, void* stream);
+
+/* Bytes of workspace qp_accumulate_attn_weights needs. */
+int64_t qp_attn_weights_workspace_bytes(int64_t num_q_tokens, int num_seqs, int num_q_heads, int num_kv_heads,
+                                        int head_size);
+
+/* Attention weight per cached key: for every sequence and KV head, the softmax weights 2^(t - lse) that the call's
+ * query rows give each cached key they see, summed over the query tokens and the query heads of the KV head, are added
+ * to weights[block, slot, KV head] (fp32; element strides weights_stride_*) of the key's cell. t is the row's scaled
+ * score in base-2 units, after the softcap; lse (tokens, q heads) fp32 is the base-2 log-sum-exp that the attention
+ * call of the same rows returned (lse_out), sinks included; a row of lse -inf adds nothing. The tokens of the call
+ * itself (keys at n - qlen + tokens_after_keys and on, n = seqused_k) have no earlier weight: theirs is stored, not
+ * added. Cells past seqused_k are left as they are. The keys of a page that several sequences of the call share get
+ * every sequence's weight, added in no fixed order. cu_seqlens_q, seqused_k, block_table, the cache, softmax_scale,
+ * q_rotated, tokens_after_keys, sliding_window and softcap as in qp_paged_decode; max_seqlen_q any length (a whole
+ * prompt, or the last chunk of one); max_seqlen_k bounds seqused_k (keys from it on are not visited). Head sizes 128,
+ * 256 and 512. No counterpart in the reference. */
+int qp_accumulate_attn_weights(int fmt, int dtype, const void* q, int64_t q_stride_token, int64_t q_stride_head,
+                               int64_t num_q_tokens, int num_seqs, const int32_t* cu_seqlens_q,
+                               const int32_t* seqused_k, int max_seqlen_q, int max_seqlen_k,
+                               const int32_t* block_table, int64_t block_table_stride, const void* cache,
+                               int block_size, int64_t block_stride, int64_t head_stride, int64_t slot_stride,
+                               int64_t k_off, int64_t ks_off, int64_t v_off, int64_t vs_off, int num_q_heads,
+                               int num_kv_heads, int head_size, float softmax_scale, const uint32_t* rht_sign_bits,
+                               int q_rotated, int tokens_after_keys, int sliding_window, float softcap,
+                               const float* lse, float* weights, int64_t weights_stride_block,
+                               int64_t weights_stride_slot, int64_t weights_stride_head, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace qp_evict_cache needs. */
+int64_t qp_evict_workspace_bytes(int num_seqs, int num_kv_heads, int max_seqlen_k, int keep);
+
+/* Eviction by accumulated attention weight: of every sequence b of n = seqused_k[b] > keep tokens, each KV head keeps
+ * its first keep_first tokens, its last keep_last and, of those between, the heaviest by `weights` (fp32, as
+ * qp_accumulate_attn_weights leaves them; of equal ones the earlier; NaN counts as lowest), keep in all. The kept
+ * cells (cell_bytes each, moved as they are) and their weights go, in order, to positions 0 .. keep - 1 of the
+ * sequence's pages; the cells behind keep their old contents. out_block_table not null: they go to those pages
+ * instead, which no sequence of the call may hold (a sequence of at most keep tokens is copied there whole), and the
+ * old pages stay as they are; null: in place, and no other sequence may share the pages. kept (seqs, KV heads, keep)
+ * gets the old position of each kept token, -1 behind the last; seqused_out (seqs; may be seqused_k itself) gets
+ * min(n, keep). Tokens from max_seqlen_k on do not exist for the call. Any cell layout with fields inside cell_bytes
+ * (a multiple of 8), strides and base multiples of 8 bytes. No counterpart in the reference. */
+int qp_evict_cache(void* cache, int cell_bytes, int block_size, int64_t block_stride, int64_t head_stride,
+                   int64_t slot_stride, int num_kv_heads, float* weights, int64_t weights_stride_block,
+                   int64_t weights_stride_slot, int64_t weights_stride_head, int num_seqs, const int32_t* seqused_k,
+                   int max_seqlen_k, const int32_t* block_table, int64_t block_table_stride,
+                   const int32_t* out_block_table, int64_t out_block_table_stride, int keep, int keep_first,
+                   int keep_last, int32_t* kept, int32_t* seqused_out, void* workspace, int64_t workspace_bytes,
+                   void* stream);
 
 #ifdef __cplusplus
 }

@@ -37,6 +37,13 @@ SIGNATURES = {
     "qp_prefill_varlen_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
     "qp_prefill_varlen": (_I, [_I, _I, _P, _L, _L, _P, _L, _L, _L, _I, _P, _P, _I, _P, _L, _P, _I, _L, _L, _L, _L, _L,
                                _L, _L, _I, _I, _I, _F, _P, _I, _I, _F, _P, _I, _P, _P, _L, _P]),
+    "qp_attn_weights_workspace_bytes": (_L, [_L, _I, _I, _I, _I]),
+    "qp_accumulate_attn_weights": (_I, [_I, _I, _P, _L, _L, _L, _I, _P, _P, _I, _I, _P, _L, _P, _I, _L, _L, _L, _L,
+                                        _L, _L, _L, _I, _I, _I, _F, _P, _I, _I, _I, _F, _P, _P, _L, _L, _L, _P, _L,
+                                        _P]),
+    "qp_evict_workspace_bytes": (_L, [_I, _I, _I, _I]),
+    "qp_evict_cache": (_I, [_P, _I, _I, _L, _L, _L, _I, _P, _L, _L, _L, _I, _P, _I, _P, _L, _P, _L, _I, _I, _I, _P, _P,
+                            _P, _L, _P]),
     "qp_peer_exchange_bytes": (_L, [_I, _L, _I, _I]),
     "qp_peer_partial_offset": (_L, [_I, _L, _I, _I, _I]),
     "qp_fold_peer_partials": (_I, [_I, _I, _L, _I, _I, _I, _P, ctypes.c_uint32, _I, _P, _L, _L, _P, _P, _P]),

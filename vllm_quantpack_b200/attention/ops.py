@@ -407,3 +407,111 @@ def prefill_varlen(q, key_cache, value_cache, out, *, cu_seqlens_q, seqused_k, m
               int(sliding_window), float(softcap or 0.0), _sinks_ptr(sinks, nq, mode), mode, lse_ptr, ws.data_ptr(),
               ws.numel() * ws.element_size(), _stream(q.device))
     return out
+
+
+# ------------------------------------------------------------------------------------------------------ eviction
+
+
+def new_attention_weights(k_scale_cache):
+    """Zeroed attention weights for a cache: fp32 (blocks, block size, KV heads) as the cache's scale views, each
+    page's weights of a KV head contiguous."""
+    nblocks, block_size, nkv = k_scale_cache.shape
+    return torch.zeros((nblocks, nkv, block_size), dtype=torch.float32, device=k_scale_cache.device).transpose(1, 2)
+
+
+def _check_device(device, **tensors):
+    """The launch goes to the current device: every tensor has to live there."""
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {device}, the current device is {torch.cuda.current_device()}")
+    for name, t in tensors.items():
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _check_weights(weights, lay):
+    if weights.dtype != torch.float32 or tuple(weights.shape) != (lay.nblocks, lay.block_size, lay.nkv):
+        raise ValueError(f"weights must be fp32 (blocks, block size, KV heads) = "
+                         f"({lay.nblocks}, {lay.block_size}, {lay.nkv}), got {weights.dtype} {tuple(weights.shape)}")
+
+
+def _check_index(**tensors):
+    for name, t in tensors.items():
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name} rows must be contiguous")
+
+
+def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_seqlens_q, max_seqlen_q, seqused_k,
+                                 max_seqlen_k, softmax_scale, block_table, k_scale_cache, v_scale_cache,
+                                 q_rotated=False, ws=None, tokens_after_keys=0, sliding_window=0, softcap=0.0):
+    """Add to `weights` (fp32 (blocks, block size, KV heads), `new_attention_weights`) the softmax weight that every
+    cached key gets from the query rows of an attention call: q, the lengths, the block table, the scale and the
+    layer's features as that call took them, `lse` the (tokens, query heads) base-2 log-sum-exp it returned in its
+    `lse_out`. Summed over the query tokens (one, or a whole prompt) and the query heads of each KV head. The call's own
+    tokens have no earlier weight: theirs is stored, so pages need no clearing before reuse as long as every token
+    enters through such a call; a first call that covers only the last tokens of a prompt wants the other cells zeroed.
+    Cells past a sequence's length are left as they are. Returns `weights`."""
+    hs, nq = q.shape[-1], q.shape[1]
+    lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
+    _check_weights(weights, lay)
+    _check_index(cu_seqlens_q=cu_seqlens_q, seqused_k=seqused_k, block_table=block_table)
+    if q.stride(-1) != 1:
+        raise ValueError("q rows must be contiguous")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], nq) or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous fp32 ({q.shape[0]}, {nq})")
+    dt = _dtype_code(q, "accumulate_attention_weights")
+    _check_device(q.device, key_cache=key_cache, weights=weights, lse=lse, cu_seqlens_q=cu_seqlens_q,
+                  seqused_k=seqused_k, block_table=block_table)
+    num_seqs = cu_seqlens_q.shape[0] - 1
+    if ws is None:
+        ws = workspace(q.device, _memo("qp_attn_weights_workspace_bytes", int(q.shape[0]), num_seqs, int(nq), lay.nkv,
+                                       int(hs)))
+    _lib.call("qp_accumulate_attn_weights", lay.fmt, dt, q.data_ptr(), q.stride(0), q.stride(1), q.shape[0], num_seqs,
+              cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q), int(max_seqlen_k),
+              block_table.data_ptr(), block_table.stride(0), *lay.args(), nq, lay.nkv, hs, float(softmax_scale),
+              rht.device_sign_bits(hs, q.device).data_ptr(), int(bool(q_rotated)), int(tokens_after_keys),
+              int(sliding_window), float(softcap or 0.0), lse.data_ptr(), weights.data_ptr(), *weights.stride(),
+              ws.data_ptr(), ws.numel() * ws.element_size(), _stream(q.device))
+    return weights
+
+
+def evict_cache(key_cache, value_cache, weights, *, seqused_k, max_seqlen_k, block_table, keep, keep_first=0,
+                keep_last=0, k_scale_cache, v_scale_cache, out_block_table=None, seqused_out=None, ws=None):
+    """Cut every sequence of more than `keep` cached tokens down to `keep`: per KV head its first `keep_first` tokens,
+    its last `keep_last` and the heaviest by `weights` in between (of equal ones the earlier). The kept cells and
+    weights move to the front of the sequence's pages, in their order, so each KV head may keep other tokens and the
+    sequence stays a sequence of min(length, keep) tokens for every call that reads it. In place (no other sequence may
+    hold the pages), or with `out_block_table` (int32 (seqs, pages)) into other pages, the old ones left as they are: a
+    sequence whose pages others share (a common prompt). Returns (kept, seqused): the old positions (seqs, KV heads,
+    keep) int32, -1 behind the last, and the new lengths (`seqused_out` if given, which may be `seqused_k` itself)."""
+    int4 = key_cache.dtype == torch.uint8
+    hs = (key_cache.shape[-1] - 4) * 2 if int4 else key_cache.shape[-1]
+    lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
+    _check_weights(weights, lay)
+    _check_index(seqused_k=seqused_k, block_table=block_table)
+    num_seqs, keep = seqused_k.shape[0], int(keep)
+    if block_table.shape[0] < num_seqs:
+        raise ValueError("block_table needs a row for every sequence")
+    if out_block_table is not None:
+        _check_index(out_block_table=out_block_table)
+        if out_block_table.shape[0] < num_seqs or out_block_table.shape[1] * lay.block_size < min(keep,
+                                                                                                   int(max_seqlen_k)):
+            raise ValueError("out_block_table needs pages for every sequence's kept tokens")
+    if seqused_out is None:
+        seqused_out = torch.empty_like(seqused_k)
+    elif seqused_out.dtype != torch.int32 or seqused_out.shape != seqused_k.shape or not seqused_out.is_contiguous():
+        raise ValueError("seqused_out must be contiguous int32, one length per sequence")
+    _check_device(key_cache.device, weights=weights, seqused_k=seqused_k, block_table=block_table,
+                  seqused_out=seqused_out, **({} if out_block_table is None else {"out_block_table": out_block_table}))
+    kept = torch.empty((num_seqs, lay.nkv, max(keep, 0)), dtype=torch.int32, device=key_cache.device)
+    if ws is None:
+        ws = workspace(key_cache.device, _memo("qp_evict_workspace_bytes", num_seqs, lay.nkv, int(max_seqlen_k), keep))
+    _lib.call("qp_evict_cache", lay.base, lay.cell, lay.block_size, lay.block_stride, lay.head_stride, lay.slot_stride,
+              lay.nkv, weights.data_ptr(), *weights.stride(), num_seqs, seqused_k.data_ptr(), int(max_seqlen_k),
+              block_table.data_ptr(), block_table.stride(0),
+              out_block_table.data_ptr() if out_block_table is not None else None,
+              out_block_table.stride(0) if out_block_table is not None else 0, keep, int(keep_first), int(keep_last),
+              kept.data_ptr(), seqused_out.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(),
+              _stream(key_cache.device))
+    return kept, seqused_out

@@ -20,6 +20,11 @@ int check_launch(const char* what);
 // Number of SMs of the current device (cached per device).
 int device_sm_count();
 
+// Checks shared by the entry points that read a cache's keys (qp_decode.cu): format, dtype, head size, cell layout.
+int decode_check_cache(const char* who, int fmt, int dtype, int head_size, const void* cache, int block_size,
+                       int64_t block_stride, int64_t head_stride, int64_t slot_stride, int64_t k_off, int64_t ks_off,
+                       int64_t v_off, int64_t vs_off);
+
 // Chunk prefill of one sequence through the split-KV decode kernel (qp_decode.cu), used by qp_prefill at head 512:
 // the arguments and outputs of qp_prefill (out_mode 0 or 1), with its own workspace size.
 int64_t decode_chunk_workspace_bytes(int qlen, int n, int num_q_heads, int num_kv_heads, int head_size);

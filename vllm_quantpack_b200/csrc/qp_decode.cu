@@ -1241,7 +1241,7 @@ extern "C" int64_t qp_decode_workspace_bytes(int64_t num_q_tokens, int num_q_hea
 }
 
 // Checks shared by the decode entry points: formats, head size, cache layout.
-static int decode_check_cache(const char* who, int fmt, int dtype, int head_size, const void* cache, int block_size,
+int decode_check_cache(const char* who, int fmt, int dtype, int head_size, const void* cache, int block_size,
                               int64_t block_stride, int64_t head_stride, int64_t slot_stride, int64_t k_off,
                               int64_t ks_off, int64_t v_off, int64_t vs_off) {
   if (fmt != FMT_INT4 && fmt != FMT_K8V4) return set_error(QP_ERR_UNSUPPORTED, "%s: format %d", who, fmt);
