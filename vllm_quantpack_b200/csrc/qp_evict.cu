@@ -5,15 +5,30 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "qp_api_internal.h"
 #include "qp_common.cuh"
 
 namespace qp {
 
+// Division of an index below 2^31 by a launch constant d: i / d = i m >> (31 + s) with s = ceil(log2 d) and
+// m = floor(2^(31 + s) / d) + 1, which fits 32 bits and is off by less than 2^s / 2^(31 + s) a unit of i.
+struct FastDiv {
+  uint32_t m;
+  int s, d;
+  explicit FastDiv(int divisor) : m(0), s(0), d(divisor) {
+    while ((1ll << s) < divisor) ++s;
+    m = static_cast<uint32_t>((1ull << (31 + s)) / static_cast<uint64_t>(divisor) + 1);
+  }
+  __device__ __forceinline__ int div(int i) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(i)) * m) >> (31 + s));
+  }
+};
+
 struct EvictParams {
   uint8_t* cache;
-  int block_size;
+  FastDiv block_size;
   int64_t block_stride, head_stride, slot_stride;  // bytes
   int cell;                                        // bytes, a multiple of 8
   float* weights;
@@ -27,6 +42,12 @@ struct EvictParams {
   int max_n, keep, first, last;
   int32_t* kept;         // [seqs][nkv][keep]: token of each kept position, -1 behind them
   int32_t* seqused_out;  // [seqs]
+  // workspace, written by the selection: new length and whether anything may move, ticket, chunk flags
+  int2* lens;       // [seqs]
+  uint32_t* ticket;
+  uint32_t* flags;  // [seqs][nkv][chunks]
+  int chunks, chunk;  // chunks of `chunk` kept positions of a pair
+  int smem_weights;   // weights a CTA of the selection holds in shared memory
 };
 
 // order of the weights as unsigned integers: NaN first (it goes first), -0 = +0
@@ -37,126 +58,292 @@ __device__ __forceinline__ uint32_t weight_rank(float x) {
 }
 
 __device__ __forceinline__ float* weight_at(const EvictParams& p, const int32_t* table, int kvh, int i) {
-  return p.weights + static_cast<int64_t>(table[i / p.block_size]) * p.w_block +
-         static_cast<int64_t>(i % p.block_size) * p.w_slot + kvh * p.w_head;
+  const int b = p.block_size.div(i);
+  return p.weights + static_cast<int64_t>(table[b]) * p.w_block +
+         static_cast<int64_t>(i - b * p.block_size.d) * p.w_slot + kvh * p.w_head;
 }
 __device__ __forceinline__ uint8_t* cell_at(const EvictParams& p, const int32_t* table, int kvh, int i) {
-  return p.cache + static_cast<int64_t>(table[i / p.block_size]) * p.block_stride +
-         static_cast<int64_t>(i % p.block_size) * p.slot_stride + static_cast<int64_t>(kvh) * p.head_stride;
+  const int b = p.block_size.div(i);
+  return p.cache + static_cast<int64_t>(table[b]) * p.block_stride +
+         static_cast<int64_t>(i - b * p.block_size.d) * p.slot_stride + static_cast<int64_t>(kvh) * p.head_stride;
 }
 
-constexpr int EV_THREADS = 1024;
-
-__device__ __forceinline__ int block_scan(int x, int* sm, int* total) {  // exclusive; all threads
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = x;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int o = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += o;
-  }
-  __syncthreads();
-  if (lane == 31) sm[warp] = incl;
-  __syncthreads();
-  int base = 0, all = 0;
-  for (int w = 0; w < EV_THREADS / 32; ++w) {
-    if (w < warp) base += sm[w];
-    all += sm[w];
-  }
-  *total = all;
-  return base + incl - x;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
+// the word at shared-memory address `p` of CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t ld_cluster(const void* p, uint32_t rank) {
+  uint32_t a, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------------------- selection
+// The threshold weight of a (sequence, KV head) by radix selection (digits of 11, 11 and 10 bits), then the kept tokens
+// in order. A cluster of 1 to 16 CTAs shares a pair: each reads its part of the weights once, from HBM into shared
+// memory (4 bytes a token are the floor of this kernel; what does not fit is read again from L2), the digits'
+// histograms and the counts meet over distributed shared memory. One launch; nothing comes back to the host.
+constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048;
+
+struct EvictShared {
+  uint32_t hist[EV_BINS];  // this CTA's
+  uint32_t bin, left;      // the digit found, and how many of its weights stay
+  uint32_t warp_sum[EV_WARPS];
+  uint32_t gt[EV_WARPS], tie[EV_WARPS];  // per warp: tokens that stay for sure, tokens at the threshold
+  uint32_t gt_all, tie_all;              // this CTA's, read by the others
+};
 
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictParams p) {
-  __shared__ int hist[256], sm[32];
-  __shared__ uint32_t sel[2];
-  const int kvh = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;");  // the move's launch may begin; it waits for this grid's end
+  extern __shared__ __align__(16) uint8_t raw[];
+  EvictShared& sh = *reinterpret_cast<EvictShared*>(raw);
+  uint32_t* ranks = reinterpret_cast<uint32_t*>(raw + sizeof(EvictShared));  // of this CTA's first smem_weights tokens
+  uint32_t rank, ctas;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  const int kvh = blockIdx.x / ctas, seq = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int32_t* table = p.table + seq * p.table_stride;
   const int n = min(max(p.seqused[seq], 0), p.max_n);
-  int32_t* kept = p.kept + (static_cast<int64_t>(seq) * p.nkv + kvh) * p.keep;
-  if (n <= p.keep) {
-    for (int j = tid; j < p.keep; j += EV_THREADS) kept[j] = j < n ? j : -1;
+  const int64_t pair = static_cast<int64_t>(seq) * p.nkv + kvh;
+  int32_t* kept = p.kept + pair * p.keep;
+  if (rank == 0) {
+    if (kvh == 0 && tid == 0) p.lens[seq] = make_int2(min(n, p.keep), n > p.keep || p.out_table != nullptr);
+    if (pair == 0 && tid == 0) *p.ticket = 0u;
+    for (int c = tid; c < p.chunks; c += EV_THREADS) p.flags[pair * p.chunks + c] = 0u;
+  }
+  if (n <= p.keep) {  // the whole cluster leaves
+    for (int j = rank * EV_THREADS + tid; j < p.keep; j += ctas * EV_THREADS) kept[j] = j < n ? j : -1;
     return;
   }
+  // this CTA's tokens
+  const int part = (n + ctas - 1) / ctas, c0 = min(static_cast<int>(rank) * part, n), c1 = min(c0 + part, n);
   const int lo = p.first, hi = n - p.last;
-  int want = p.keep - p.first - p.last;  // of [lo, hi)
-  uint32_t thr = 0, mask = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += EV_THREADS) hist[i] = 0;
+  const auto rank_of = [&](int i) {
+    const int k = i - c0;
+    return k < p.smem_weights ? ranks[k] : weight_rank(*weight_at(p, table, kvh, i));
+  };
+#pragma unroll 4
+  for (int i = c0 + tid; i < min(c1, c0 + p.smem_weights); i += EV_THREADS)
+    ranks[i - c0] = weight_rank(*weight_at(p, table, kvh, i));
+
+  uint32_t thr = 0, mask = 0, want = p.keep - p.first - p.last;  // of the tokens [lo, hi)
+  const int b0 = max(c0, lo), b1 = min(c1, hi);
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : EV_BINS;
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) sh.hist[i] = 0;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += EV_THREADS) {
-      const uint32_t r = weight_rank(*weight_at(p, table, kvh, i));
-      if ((r & mask) == thr) atomicAdd(&hist[(r >> shift) & 255], 1);
+    for (int i = b0 + tid; i < b1; i += EV_THREADS) {
+      const uint32_t r = rank_of(i);
+      if ((r & mask) == thr) atomicAdd(&sh.hist[(r >> shift) & (bins - 1)], 1u);
     }
-    __syncthreads();
-    if (tid == 0) {
-      int b = 255, left = want;
-      while (b > 0 && hist[b] < left) left -= hist[b--];
-      sel[0] = b;
-      sel[1] = left;
+    cluster_sync();
+    // every CTA adds the histograms up (4 bins a thread, the highest first) and finds the digit
+    uint32_t h[4], sum = 0;
+    const int top = EV_BINS - 1 - 4 * tid;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[k] = 0;
+      for (uint32_t c = 0; c < ctas; ++c) h[k] += ld_cluster(&sh.hist[top - k], c);
+      sum += h[k];
     }
+    uint32_t incl = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    if (lane == 31) sh.warp_sum[warp] = incl;
     __syncthreads();
-    thr |= sel[0] << shift;
-    mask |= 255u << shift;
-    want = sel[1];
-    __syncthreads();
+    uint32_t above = incl - sum;
+    for (int w = 0; w < warp; ++w) above += sh.warp_sum[w];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // the bin in which the want-th heaviest lies (want = 0: none, all bits stay 1)
+      if (above < want && want <= above + h[k]) {
+        sh.bin = top - k;
+        sh.left = want - above;
+      }
+      above += h[k];
+    }
+    if (want == 0 && tid == 0) {
+      sh.bin = bins - 1;
+      sh.left = 0;
+    }
+    cluster_sync();  // the others have read this CTA's histogram too
+    thr |= sh.bin << shift;
+    mask |= static_cast<uint32_t>(bins - 1) << shift;
+    want = sh.left;
   }
-  // want of the weights equal to the threshold stay, the earliest ones
-  int eq = 0, out = 0;
-  for (int i0 = 0; i0 < n; i0 += EV_THREADS) {
-    const int i = i0 + tid;
-    bool stay = i < n && (i < lo || i >= hi), tie = false;
-    if (i < n && !stay) {
-      const uint32_t r = weight_rank(*weight_at(p, table, kvh, i));
-      stay = r > thr;
-      tie = r == thr;
-    }
-    int total;
-    const int rank = block_scan(tie, sm, &total);
-    if (tie && eq + rank < want) stay = true;
-    eq += total;
-    const int at = block_scan(stay, sm, &total);
-    if (stay) kept[out + at] = i;
-    out += total;
+  // Tokens above the threshold stay, and of those at it the first `want`. Each warp takes a run of tokens: it counts,
+  // the counts are summed over the warps and the CTAs before it, and it writes its tokens in order.
+  const int run = (part + EV_WARPS - 1) / EV_WARPS, w0 = min(c0 + warp * run, c1), w1 = min(w0 + run, c1);
+  uint32_t gt = 0, tie = 0;
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const bool sure = i < lo || i >= hi;
+    const uint32_t r = sure ? 0u : rank_of(i);
+    gt += sure || r > thr;
+    tie += !sure && r == thr;
   }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, d);
+    tie += __shfl_xor_sync(0xffffffffu, tie, d);
+  }
+  if (lane == 0) {
+    sh.gt[warp] = gt;
+    sh.tie[warp] = tie;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t g = 0, t = 0;
+    for (int w = 0; w < EV_WARPS; ++w) {
+      g += sh.gt[w];
+      t += sh.tie[w];
+    }
+    sh.gt_all = g;
+    sh.tie_all = t;
+  }
+  cluster_sync();
+  gt = tie = 0;
+  for (uint32_t c = 0; c < rank; ++c) {
+    gt += ld_cluster(&sh.gt_all, c);
+    tie += ld_cluster(&sh.tie_all, c);
+  }
+  for (int w = 0; w < warp; ++w) {
+    gt += sh.gt[w];
+    tie += sh.tie[w];
+  }
+  uint32_t at = gt + min(tie, want);
+  const uint32_t below = (1u << lane) - 1u;
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int i = i0 + lane;
+    const bool in = i < w1, sure = in && (i < lo || i >= hi);
+    const uint32_t r = in && !sure ? rank_of(i) : 0u;
+    const bool eq = in && !sure && r == thr;
+    const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
+    const bool stay = sure || (in && !sure && r > thr) || (eq && tie + __popc(eqs & below) < want);
+    const uint32_t stays = __ballot_sync(0xffffffffu, stay);
+    if (stay) kept[at + __popc(stays & below)] = i;
+    at += __popc(stays);
+    tie += __popc(eqs);
+  }
+  cluster_sync();  // no CTA leaves while another may still read its counts
 }
 
-// One CTA per (KV head, sequence), 64 cells at a time: a position's token is never before it, so what a tile overwrites
-// has been read by then.
-__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
-  extern __shared__ __align__(16) uint8_t buf[];
-  const int kvh = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+// ---------------------------------------------------------------------------------------------------- move
+// The kept cells to their places, `chunk` positions of a pair at a time, each cell read once and written once. In place,
+// position j gets token kept[j] >= j, so the cells a chunk overwrites are wanted by chunks before it at most: a CTA
+// reads its cells into shared memory, says so in its flag, and before it writes waits (bounded) for the chunks that take
+// a cell from its range. Chunks are handed out by a ticket, a pair's lower ones first, so those it waits for have been
+// taken by CTAs that run already and wait for still lower ones only.
+constexpr int MV_THREADS = 256;
+
+__device__ __forceinline__ int lower_bound(const int32_t* kept, int len, int token) {
+  int lo = 0, hi = len;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (kept[mid] < token) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(MV_THREADS) evict_move_kernel(const EvictParams p, const FastDiv words) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  extern __shared__ __align__(16) uint8_t raw[];
+  __shared__ uint32_t ticket;
+  const int tid = threadIdx.x;
+  uint2* cells = reinterpret_cast<uint2*>(raw);
+  const uint8_t** src = reinterpret_cast<const uint8_t**>(raw + p.chunk * p.cell);  // null: nothing to move
+  uint8_t** dst = const_cast<uint8_t**>(src) + p.chunk;
+  if (tid == 0) ticket = atomicAdd(p.ticket, 1u);
+  __syncthreads();
+  const int pairs = p.num_seqs * p.nkv, chunk = ticket / pairs, pair = ticket % pairs;
+  const int seq = pair / p.nkv, kvh = pair % p.nkv;
+  const int2 len = p.lens[seq];
+  if (chunk == 0 && kvh == 0 && tid == 0) p.seqused_out[seq] = len.x;
+  const int j0 = chunk * p.chunk, m = min(p.chunk, len.x - j0);
+  if (m <= 0 || !len.y) return;
   const int32_t* from = p.table + seq * p.table_stride;
   const int32_t* to = p.out_table ? p.out_table + seq * p.out_stride : from;
-  const int32_t* kept = p.kept + (static_cast<int64_t>(seq) * p.nkv + kvh) * p.keep;
-  const int words = p.cell / 8;
-  uint2* cells = reinterpret_cast<uint2*>(buf);
-  float* w = reinterpret_cast<float*>(buf + 64 * p.cell);
-  for (int j0 = 0; j0 < p.keep; j0 += 64) {
-    const int m = min(64, p.keep - j0);
-    for (int e = tid; e < m * words; e += 256) {
-      const int i = kept[j0 + e / words];
-      if (i >= 0) cells[e] = reinterpret_cast<const uint2*>(cell_at(p, from, kvh, i))[e % words];
+  const int32_t* kept = p.kept + static_cast<int64_t>(pair) * p.keep;
+  float w = 0.f;
+  float* w_to = nullptr;
+  bool moves = false;
+  for (int k = tid; k < m; k += MV_THREADS) {  // at most one a thread: chunk <= MV_THREADS
+    const int i = kept[j0 + k];
+    moves = p.out_table != nullptr || i != j0 + k;
+    src[k] = moves ? cell_at(p, from, kvh, i) : nullptr;
+    dst[k] = cell_at(p, to, kvh, j0 + k);
+    if (moves) {
+      w = *weight_at(p, from, kvh, i);
+      w_to = weight_at(p, to, kvh, j0 + k);
     }
-    if (tid < m && kept[j0 + tid] >= 0) w[tid] = *weight_at(p, from, kvh, kept[j0 + tid]);
-    __syncthreads();
-    for (int e = tid; e < m * words; e += 256)
-      if (kept[j0 + e / words] >= 0) reinterpret_cast<uint2*>(cell_at(p, to, kvh, j0 + e / words))[e % words] = cells[e];
-    if (tid < m && kept[j0 + tid] >= 0) *weight_at(p, to, kvh, j0 + tid) = w[tid];
-    __syncthreads();
   }
+  if (!__syncthreads_or(moves)) return;  // nobody else takes a cell from a range that stays
+  const int total = m * words.d;
+#pragma unroll 8
+  for (int e = tid; e < total; e += MV_THREADS) {
+    const int k = words.div(e);
+    const uint8_t* s = src[k];
+    if (s != nullptr) cells[e] = reinterpret_cast<const uint2*>(s)[e - k * words.d];
+  }
+  bool ok = true;
+  if (p.out_table == nullptr) {
+    // this CTA's reads are done (their values are in shared memory, the weight in the word below)
+    uint32_t* flags = p.flags + static_cast<int64_t>(pair) * p.chunks;
+    __shared__ float w_seen[MV_THREADS];
+    w_seen[tid] = w;
+    __syncthreads();
+    w = w_seen[tid];
+    if (tid == 0) {
+      __threadfence();
+      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flags + chunk), "r"(1u) : "memory");
+    }
+    // tokens [j0, j0 + m) lie at kept positions [r0, r1) of chunks up to this one
+    const int r0 = lower_bound(kept, len.x, j0), r1 = lower_bound(kept, len.x, j0 + m);
+    for (int c = r0 / p.chunk + tid; r1 > r0 && c <= (r1 - 1) / p.chunk && c < chunk; c += MV_THREADS) {
+      const uint64_t t0 = global_timer_ns();
+      uint32_t v;
+      do {
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flags + c) : "memory");
+        if (v == 0u && global_timer_ns() - t0 > 2000000000ull) {
+          atomicCAS(&g_device_error, DEV_ERR_NONE, DEV_ERR_WAIT_TIMEOUT);
+          ok = false;
+        }
+      } while (v == 0u && ok);
+    }
+  }
+  if (__syncthreads_or(!ok)) return;
+#pragma unroll 8
+  for (int e = tid; e < total; e += MV_THREADS) {
+    const int k = words.div(e);
+    if (src[k] != nullptr) reinterpret_cast<uint2*>(dst[k])[e - k * words.d] = cells[e];
+  }
+  if (w_to != nullptr) *w_to = w;
 }
 
-__global__ void evict_lens_kernel(const EvictParams p) {
-  const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b < p.num_seqs) p.seqused_out[b] = min(min(max(p.seqused[b], 0), p.max_n), p.keep);
+// CTAs of a pair's cluster: about EV_PART tokens each, 16 at most
+constexpr int EV_PART = 8192;
+static int evict_cluster(int max_n) {
+  int c = 1;
+  while (c < 16 && c * EV_PART < max_n) c *= 2;
+  return c;
 }
+// Kept positions a CTA of the move takes: 16 to 24 KB of cells
+static int evict_chunk(int cell) { return cell <= 200 ? 128 : cell <= 392 ? 64 : 32; }
 
 }  // namespace qp
 
 using namespace qp;
 
-extern "C" int64_t qp_evict_workspace_bytes(int num_seqs, int num_kv_heads, int max_seqlen_k, int keep) { return 256; }
+// [int2 lens (seqs)][ticket, 16 bytes][uint32 flags: one a chunk of every pair], the chunks counted at their smallest
+extern "C" int64_t qp_evict_workspace_bytes(int num_seqs, int num_kv_heads, int max_seqlen_k, int keep) {
+  if (num_seqs <= 0 || num_kv_heads <= 0 || keep <= 0) return 256;
+  const int64_t chunks = (std::min(keep, std::max(max_seqlen_k, 1)) + 31) / 32;
+  return (num_seqs * 8ll + 15) / 16 * 16 + 16 + static_cast<int64_t>(num_seqs) * num_kv_heads * chunks * 4 + 256;
+}
 
 extern "C" int qp_evict_cache(void* cache, int cell_bytes, int block_size, int64_t block_stride, int64_t head_stride,
                               int64_t slot_stride, int num_kv_heads, float* weights, int64_t weights_stride_block,
@@ -182,23 +369,50 @@ extern "C" int qp_evict_cache(void* cache, int cell_bytes, int block_size, int64
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)
     return set_error(QP_ERR_WORKSPACE, "evict: workspace of %lld bytes < %lld", (long long)workspace_bytes,
                      (long long)need);
-  const EvictParams p{static_cast<uint8_t*>(cache), block_size, block_stride, head_stride, slot_stride, cell_bytes,
-                      weights, weights_stride_block, weights_stride_slot, weights_stride_head, num_kv_heads, num_seqs,
-                      seqused_k, block_table, block_table_stride, out_block_table, out_block_table_stride, max_seqlen_k,
-                      keep, keep_first, keep_last, kept, seqused_out};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(num_seqs));
-  evict_select_kernel<<<grid, EV_THREADS, 0, st>>>(p);
-  int rc = check_launch("evict select");
-  if (rc) return rc;
-  const int smem = 64 * cell_bytes + 64 * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int chunk = evict_chunk(cell_bytes);
+  const int chunks = (std::min(keep, std::max(max_seqlen_k, 1)) + chunk - 1) / chunk;
+  const int64_t tickets = static_cast<int64_t>(num_seqs) * num_kv_heads * chunks;
+  if (tickets > 0x7fffffff) return set_error(QP_ERR_UNSUPPORTED, "evict: grid too large");
+  const int cluster = evict_cluster(max_seqlen_k);
+  const int part = (max_seqlen_k + cluster - 1) / cluster;
+  const int held = std::min(part, 48 * 1024);
+  int2* lens = static_cast<int2*>(workspace);
+  uint32_t* ticket = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + (num_seqs * 8ll + 15) / 16 * 16);
+  const EvictParams p{static_cast<uint8_t*>(cache), FastDiv(block_size), block_stride, head_stride, slot_stride,
+                      cell_bytes, weights, weights_stride_block, weights_stride_slot, weights_stride_head,
+                      num_kv_heads, num_seqs, seqused_k, block_table, block_table_stride, out_block_table,
+                      out_block_table_stride, max_seqlen_k, keep, keep_first, keep_last, kept, seqused_out, lens,
+                      ticket, ticket + 4, chunks, chunk, held};
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(sizeof(EvictShared)) + 48 * 1024 * 4);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "evict attribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
-  evict_move_kernel<<<grid, 256, smem, st>>>(p);
-  rc = check_launch("evict move");
-  if (rc) return rc;
-  evict_lens_kernel<<<(num_seqs + 255) / 256, 256, 0, st>>>(p);
-  return check_launch("evict lengths");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(num_kv_heads * cluster), static_cast<unsigned>(num_seqs));
+  cfg.blockDim = dim3(EV_THREADS);
+  cfg.dynamicSmemBytes = sizeof(EvictShared) + static_cast<size_t>(held) * 4;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
+  if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "evict select launch: %s", cudaGetErrorString(e));
+  cfg.gridDim = dim3(static_cast<unsigned>(tickets));
+  cfg.blockDim = dim3(MV_THREADS);
+  cfg.dynamicSmemBytes = static_cast<size_t>(chunk) * (cell_bytes + 2 * sizeof(void*));
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, p, FastDiv(cell_bytes / 8));
+  if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "evict move launch: %s", cudaGetErrorString(e));
+  return QP_OK;
 }
