@@ -79,15 +79,22 @@ __device__ __forceinline__ uint32_t ld_cluster(const void* p, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ void add_cluster(void* p, uint32_t rank, uint32_t v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------------- selection
 // The threshold weight of a (sequence, KV head) by radix selection (digits of 11, 11 and 10 bits), then the kept tokens
 // in order. A cluster of 1 to 16 CTAs shares a pair: each reads its part of the weights once, from HBM into shared
 // memory (4 bytes a token are the floor of this kernel; what does not fit is read again from L2), the digits'
 // histograms and the counts meet over distributed shared memory. One launch; nothing comes back to the host.
-constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048;
+constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048;
 
 struct EvictShared {
-  uint32_t hist[EV_BINS];  // this CTA's
+  uint32_t hist[EV_BINS];   // this CTA's
+  uint32_t total[EV_BINS];  // in the first CTA: the cluster's
   uint32_t bin, left;      // the digit found, and how many of its weights stay
   uint32_t warp_sum[EV_WARPS];
   uint32_t gt[EV_WARPS], tie[EV_WARPS];  // per warp: tokens that stay for sure, tokens at the threshold
@@ -102,6 +109,10 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
   uint32_t rank, ctas;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  const auto sync = [&]() {
+    if (ctas == 1) __syncthreads();
+    else cluster_sync();
+  };
   const int kvh = blockIdx.x / ctas, seq = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int32_t* table = p.table + seq * p.table_stride;
   const int n = min(max(p.seqused[seq], 0), p.max_n);
@@ -123,7 +134,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     const int k = i - c0;
     return k < p.smem_weights ? ranks[k] : weight_rank(*weight_at(p, table, kvh, i));
   };
-#pragma unroll 4
+#pragma unroll 8
   for (int i = c0 + tid; i < min(c1, c0 + p.smem_weights); i += EV_THREADS)
     ranks[i - c0] = weight_rank(*weight_at(p, table, kvh, i));
 
@@ -132,48 +143,49 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : EV_BINS;
-    for (int i = tid; i < EV_BINS; i += EV_THREADS) sh.hist[i] = 0;
-    __syncthreads();
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) sh.hist[i] = sh.total[i] = 0;
+    sync();
     for (int i = b0 + tid; i < b1; i += EV_THREADS) {
       const uint32_t r = rank_of(i);
       if ((r & mask) == thr) atomicAdd(&sh.hist[(r >> shift) & (bins - 1)], 1u);
     }
-    cluster_sync();
-    // every CTA adds the histograms up (4 bins a thread, the highest first) and finds the digit
-    uint32_t h[4], sum = 0;
-    const int top = EV_BINS - 1 - 4 * tid;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[k] = 0;
-      for (uint32_t c = 0; c < ctas; ++c) h[k] += ld_cluster(&sh.hist[top - k], c);
-      sum += h[k];
-    }
-    uint32_t incl = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += v;
-    }
-    if (lane == 31) sh.warp_sum[warp] = incl;
     __syncthreads();
-    uint32_t above = incl - sum;
-    for (int w = 0; w < warp; ++w) above += sh.warp_sum[w];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {  // the bin in which the want-th heaviest lies (want = 0: none, all bits stay 1)
-      if (above < want && want <= above + h[k]) {
-        sh.bin = top - k;
-        sh.left = want - above;
+    for (int i = tid; i < EV_BINS; i += EV_THREADS)  // few bins hold anything
+      if (sh.hist[i] != 0u) {
+        if (rank == 0) atomicAdd(&sh.total[i], sh.hist[i]);
+        else add_cluster(&sh.total[i], 0, sh.hist[i]);
       }
-      above += h[k];
+    sync();
+    if (rank == 0) {  // the bin in which the want-th heaviest lies, from the highest on (2 bins a thread)
+      const int top = EV_BINS - 1 - 2 * tid;
+      const uint32_t h0 = sh.total[top], h1 = sh.total[top - 1];
+      uint32_t incl = h0 + h1;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += v;
+      }
+      if (lane == 31) sh.warp_sum[warp] = incl;
+      __syncthreads();
+      uint32_t before = sh.warp_sum[lane];  // EV_WARPS = 32
+      before = __reduce_add_sync(0xffffffffu, lane < warp ? before : 0u);
+      const uint32_t above = before + incl - h0 - h1;
+      if (above < want && want <= above + h0) {
+        sh.bin = top;
+        sh.left = want - above;
+      } else if (above + h0 < want && want <= above + h0 + h1) {
+        sh.bin = top - 1;
+        sh.left = want - above - h0;
+      }
+      if (want == 0 && tid == 0) {  // none stays: all bits 1, above every weight
+        sh.bin = bins - 1;
+        sh.left = 0;
+      }
     }
-    if (want == 0 && tid == 0) {
-      sh.bin = bins - 1;
-      sh.left = 0;
-    }
-    cluster_sync();  // the others have read this CTA's histogram too
-    thr |= sh.bin << shift;
+    sync();
+    thr |= ld_cluster(&sh.bin, 0) << shift;
     mask |= static_cast<uint32_t>(bins - 1) << shift;
-    want = sh.left;
+    want = ld_cluster(&sh.left, 0);
   }
   // Tokens above the threshold stay, and of those at it the first `want`. Each warp takes a run of tokens: it counts,
   // the counts are summed over the warps and the CTAs before it, and it writes its tokens in order.
@@ -204,7 +216,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     sh.gt_all = g;
     sh.tie_all = t;
   }
-  cluster_sync();
+  sync();
   gt = tie = 0;
   for (uint32_t c = 0; c < rank; ++c) {
     gt += ld_cluster(&sh.gt_all, c);
@@ -228,7 +240,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     at += __popc(stays);
     tie += __popc(eqs);
   }
-  cluster_sync();  // no CTA leaves while another may still read its counts
+  sync();  // no CTA leaves while another may still read its counts
 }
 
 // ---------------------------------------------------------------------------------------------------- move
@@ -237,7 +249,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
 // reads its cells into shared memory, says so in its flag, and before it writes waits (bounded) for the chunks that take
 // a cell from its range. Chunks are handed out by a ticket, a pair's lower ones first, so those it waits for have been
 // taken by CTAs that run already and wait for still lower ones only.
-constexpr int MV_THREADS = 256;
+constexpr int MV_THREADS = 256, MV_BATCH = 7, MV_CTAS = 6;  // 86 KB in flight an SM
 
 __device__ __forceinline__ int lower_bound(const int32_t* kept, int len, int token) {
   int lo = 0, hi = len;
@@ -249,17 +261,20 @@ __device__ __forceinline__ int lower_bound(const int32_t* kept, int len, int tok
   return lo;
 }
 
-__global__ void __launch_bounds__(MV_THREADS) evict_move_kernel(const EvictParams p, const FastDiv words) {
+__global__ void __launch_bounds__(MV_THREADS, MV_CTAS) evict_move_kernel(const EvictParams p, const FastDiv words) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ __align__(16) uint8_t raw[];
   __shared__ uint32_t ticket;
   const int tid = threadIdx.x;
-  uint2* cells = reinterpret_cast<uint2*>(raw);
-  const uint8_t** src = reinterpret_cast<const uint8_t**>(raw + p.chunk * p.cell);  // null: nothing to move
-  uint8_t** dst = const_cast<uint8_t**>(src) + p.chunk;
-  if (tid == 0) ticket = atomicAdd(p.ticket, 1u);
-  __syncthreads();
-  const int pairs = p.num_seqs * p.nkv, chunk = ticket / pairs, pair = ticket % pairs;
+  const uint8_t** src = reinterpret_cast<const uint8_t**>(raw);  // of each position; null: it stays
+  uint8_t** dst = reinterpret_cast<uint8_t**>(raw) + p.chunk;
+  uint2* cells = reinterpret_cast<uint2*>(dst + p.chunk);  // in place only
+  if (p.out_table == nullptr) {
+    if (tid == 0) ticket = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+  }
+  const int unit = p.out_table ? blockIdx.x : ticket;
+  const int pairs = p.num_seqs * p.nkv, chunk = unit / pairs, pair = unit % pairs;
   const int seq = pair / p.nkv, kvh = pair % p.nkv;
   const int2 len = p.lens[seq];
   if (chunk == 0 && kvh == 0 && tid == 0) p.seqused_out[seq] = len.x;
@@ -282,15 +297,38 @@ __global__ void __launch_bounds__(MV_THREADS) evict_move_kernel(const EvictParam
     }
   }
   if (!__syncthreads_or(moves)) return;  // nobody else takes a cell from a range that stays
+  // 8 bytes a lane (cells are 8-byte aligned), MV_BATCH of them in flight; the pointers come out of shared memory before
+  // anything is written there
   const int total = m * words.d;
-#pragma unroll 8
-  for (int e = tid; e < total; e += MV_THREADS) {
-    const int k = words.div(e);
-    const uint8_t* s = src[k];
-    if (s != nullptr) cells[e] = reinterpret_cast<const uint2*>(s)[e - k * words.d];
+  const auto batch = [&](int e0, auto&& store) {
+    uint2 v[MV_BATCH];
+    uint32_t has = 0;
+#pragma unroll
+    for (int u = 0; u < MV_BATCH; ++u) {
+      const int e = e0 + u * MV_THREADS + tid, k = words.div(e);
+      const uint8_t* from_cell = e < total ? src[k] : nullptr;
+      if (from_cell != nullptr) {
+        has |= 1u << u;
+        v[u] = __ldcs(reinterpret_cast<const uint2*>(from_cell) + (e - k * words.d));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < MV_BATCH; ++u)
+      if (has & (1u << u)) store(e0 + u * MV_THREADS + tid, v[u]);
+  };
+  if (p.out_table != nullptr) {  // nothing that is written is read by anyone
+    for (int e0 = 0; e0 < total; e0 += MV_BATCH * MV_THREADS)
+      batch(e0, [&](int e, const uint2& v) {
+        const int k = words.div(e);
+        reinterpret_cast<uint2*>(dst[k])[e - k * words.d] = v;
+      });
+    if (w_to != nullptr) *w_to = w;
+    return;
   }
+  for (int e0 = 0; e0 < total; e0 += MV_BATCH * MV_THREADS)
+    batch(e0, [&](int e, const uint2& v) { cells[e] = v; });
   bool ok = true;
-  if (p.out_table == nullptr) {
+  {
     // this CTA's reads are done (their values are in shared memory, the weight in the word below)
     uint32_t* flags = p.flags + static_cast<int64_t>(pair) * p.chunks;
     __shared__ float w_seen[MV_THREADS];
@@ -325,7 +363,7 @@ __global__ void __launch_bounds__(MV_THREADS) evict_move_kernel(const EvictParam
 }
 
 // CTAs of a pair's cluster: about EV_PART tokens each, 16 at most
-constexpr int EV_PART = 8192;
+constexpr int EV_PART = 16384;
 static int evict_cluster(int max_n) {
   int c = 1;
   while (c < 16 && c * EV_PART < max_n) c *= 2;
@@ -409,7 +447,7 @@ extern "C" int qp_evict_cache(void* cache, int cell_bytes, int block_size, int64
   if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "evict select launch: %s", cudaGetErrorString(e));
   cfg.gridDim = dim3(static_cast<unsigned>(tickets));
   cfg.blockDim = dim3(MV_THREADS);
-  cfg.dynamicSmemBytes = static_cast<size_t>(chunk) * (cell_bytes + 2 * sizeof(void*));
+  cfg.dynamicSmemBytes = static_cast<size_t>(chunk) * (2 * sizeof(void*) + (out_block_table ? 0 : cell_bytes));
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   e = cudaLaunchKernelEx(&cfg, evict_move_kernel, p, FastDiv(cell_bytes / 8));
