@@ -233,8 +233,8 @@ int qp_merge_attn_partials(int dtype, int head_size, int64_t num_tokens, int num
                            const uint32_t* rht_sign_bits, void* stream);
 
 /* Bytes of workspace qp_accumulate_attn_weights needs. */
-int64_t qp_attn_weights_workspace_bytes(int64_t num_q_tokens, int num_seqs, int num_q_heads, int num_kv_heads,
-                                        int head_size);
+int64_t qp_attn_weights_workspace_bytes(int64_t num_q_tokens, int num_seqs, int max_seqlen_q, int num_q_heads,
+                                        int num_kv_heads, int head_size);
 
 /* Attention weight per cached key: for every sequence and KV head, the softmax weights 2^(t - lse) that the call's
  * query rows give each cached key they see, summed over the query tokens and the query heads of the KV head, are added

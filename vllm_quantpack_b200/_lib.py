@@ -37,7 +37,7 @@ SIGNATURES = {
     "qp_prefill_varlen_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
     "qp_prefill_varlen": (_I, [_I, _I, _P, _L, _L, _P, _L, _L, _L, _I, _P, _P, _I, _P, _L, _P, _I, _L, _L, _L, _L, _L,
                                _L, _L, _I, _I, _I, _F, _P, _I, _I, _F, _P, _I, _P, _P, _L, _P]),
-    "qp_attn_weights_workspace_bytes": (_L, [_L, _I, _I, _I, _I]),
+    "qp_attn_weights_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
     "qp_accumulate_attn_weights": (_I, [_I, _I, _P, _L, _L, _L, _I, _P, _P, _I, _I, _P, _L, _P, _I, _L, _L, _L, _L,
                                         _L, _L, _L, _I, _I, _I, _F, _P, _I, _I, _I, _F, _P, _P, _L, _L, _L, _P, _L,
                                         _P]),

@@ -465,8 +465,8 @@ def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_
                   seqused_k=seqused_k, block_table=block_table)
     num_seqs = cu_seqlens_q.shape[0] - 1
     if ws is None:
-        ws = workspace(q.device, _memo("qp_attn_weights_workspace_bytes", int(q.shape[0]), num_seqs, int(nq), lay.nkv,
-                                       int(hs)))
+        ws = workspace(q.device, _memo("qp_attn_weights_workspace_bytes", int(q.shape[0]), num_seqs,
+                                       int(max_seqlen_q), int(nq), lay.nkv, int(hs)))
     _lib.call("qp_accumulate_attn_weights", lay.fmt, dt, q.data_ptr(), q.stride(0), q.stride(1), q.shape[0], num_seqs,
               cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q), int(max_seqlen_k),
               block_table.data_ptr(), block_table.stride(0), *lay.args(), nq, lay.nkv, hs, float(softmax_scale),

@@ -3,115 +3,882 @@
 //   t_ik = (softmax_scale / hs) log2(e) q_i . k_k      (RHT domain; softcap and sliding window as in the attention)
 // with lse the base-2 log-sum-exp the attention call returned for the row, so the weights a row hands out sum to one
 // (less what a sink took). A key a row does not see gets nothing from it.
+//
+// The result is fp32, and its relative error is the score's absolute one: a query row rounded to fp16 (2^-12 of a
+// score of several units) would leave three digits. So a row enters as the sum of two fp16 terms (2^-22; K4q writes
+// them with the RHT applied) and a score takes twice the products; the key codes are exact (u - zp, int8).
+//
+// The keys are the M of the MMA and the query rows its N, so a key is a TMEM lane and its sum over rows stays in one
+// thread:  S^T (128 keys x N rows) = K_op (TMEM) x [Q_hi; Q_lo]^T (shared memory)  ->  sum_n 2^(k_scale S + ...)
+// One persistent CTA per SM; roles:
+//   warp 0        query tiles: one bulk copy of a prepared record (both terms in the operand's swizzled layout, the
+//                 rows' -lse and mask bounds) into a ring; a tile that the next keys use again is not copied again;
+//   warp 1        issues HS / 8 MMAs of K 16 per 128 keys and query tile, S^T double-buffered;
+//   warps 2-5     keys: cp.async of the key half of the cells only, 8 bytes a lane (the values in between are not
+//                 read: a cell's key part is not 16-byte aligned), then thread = key: codes to exact fp16 in TMEM;
+//   warps 6-13    thread = key and half of the columns: exponentials, the sum, one add to global memory per key.
+// Few rows (up to 32, decoding): a tile of 128 keys meets one query tile, two key tiles alternate in TMEM; bound by
+// the bytes of the key half (136 of 264 at int4, head 256). Many rows (prompts): a group of two key tiles stays in
+// TMEM while all query tiles that see it stream through L2, so a query tile's bytes serve 256 keys; bound by the MMAs
+// (two terms) at head 256, by the exponentials (16 a cycle and SM) at head 128.
+// The (key group, query tile) steps of all sequences and KV heads are cut evenly over the CTAs; where a cut falls
+// inside a group its parts go to the workspace and K4f adds them in order, so the sum does not depend on timing.
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "qp_api_internal.h"
 #include "qp_common.cuh"
 #include "qp_decode.cuh"
+#include "qp_tcgen05.cuh"
 
 namespace qp {
 
 struct WeightParams {
-  DecodeParams d;      // queries, lengths, block table, cache, features (num_splits and the partials unused)
-  const float* lse;    // [tokens][nq]
+  DecodeParams d;    // queries, lengths, block table, cache, features (num_splits and the partials unused)
+  const float* lse;  // [tokens][nq]
   float* weights;
   int64_t w_block, w_slot, w_head;  // element strides
-  int head_size;
+  int max_q, max_k;  // bounds of the lengths that the launch was sized for
+  // workspace: prepared query tiles; per CTA the sums of a group's parts and what they are
+  uint8_t* qrec;
+  float* part;    // [CTAs][2][256]: a group begun by an earlier CTA, a group that goes on in the next
+  int4* records;  // [CTAs][2]: {valid, goes on}, {valid, sequence, KV head, group}
 };
 
-// One thread a key, the query rows rotated into shared memory one by one.
-template <int FMT, int DT, int HS>
-__global__ void __launch_bounds__(128) weights_kernel(const WeightParams wp) {
-  const DecodeParams& p = wp.d;
-  using EL = Elem<DT>;
+constexpr int WT_KEYS = 128;     // keys of a tile (TMEM lanes)
+constexpr int WT_THREADS = 448;  // 14 warps
+constexpr int WT_SMALL_ROWS = 32;  // query rows of a KV head up to which a sequence is one query tile
+
+// NR: rows of a query tile; KT: key tiles of a group; MANY: a sequence may have several query tiles
+template <int FMT, int HS, int NR, int KT, bool MANY>
+struct WT {
   using CL = Cell<FMT, HS>;
-  constexpr int E = HS / 32;
-  __shared__ float qrow[8][HS];
-  __shared__ float row_lse[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
-  const DecodeSpan sp = decode_span(p, blockIdx.z);
-  const int key = blockIdx.x * 128 + threadIdx.x;
-  if (sp.qlen <= 0 || blockIdx.x * 128 >= sp.n) return;
-  const bool valid = key < sp.n;
-  const uint8_t* cell = nullptr;
-  float ks = 0.f, zp = 0.f;
-  int64_t at = 0;
-  if (valid) {
-    const int64_t blk = sp.btab[key / p.block_size];
-    cell = p.cache + blk * p.block_stride + static_cast<int64_t>(kvh) * p.head_stride +
-           static_cast<int64_t>(key % p.block_size) * CL::BYTES;
-    at = blk * wp.w_block + static_cast<int64_t>(key % p.block_size) * wp.w_slot + kvh * wp.w_head;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(cell + CL::KS);
-    ks = __uint_as_float(FMT == FMT_INT4 ? w & 0xFFFFFFF0u : w);
-    zp = FMT == FMT_INT4 ? static_cast<float>(w & 0xFu) : 0.f;
+  static constexpr int SLOTS = HS == 512 ? 1 : 2;  // key tiles in TMEM
+  static constexpr int ACOLS = HS / 2;             // TMEM columns of one
+  static constexpr int S = SLOTS * ACOLS;          // S^T: two buffers of NR columns
+  static constexpr int COLS = S + 2 * NR <= 256 ? 256 : 512;
+  static_assert(KT <= SLOTS && S + 2 * NR <= 512, "TMEM");
+  static constexpr int PIECES = CL::KB / 8 + 1;    // 8-byte pieces of a key's codes and scale
+  static constexpr int KEY = PIECES * 8;           // bytes of a key in a raw stage (an odd multiple of 8: no conflicts)
+  static constexpr int STAGE = WT_KEYS * KEY;
+  static constexpr int ATOM = NR * 128;            // 64 channels of a query tile's term
+  static constexpr int TERM = HS / 64 * ATOM;
+  static constexpr int ROWS = 2 * TERM;            // then [NR] float -lse, [NR] int last key, [NR] int first key,
+  static constexpr int HEAD = ROWS + 12 * NR;      // then {score scale, least last key, greatest first key}
+  static constexpr int QREC = (HEAD + 16 + 1023) / 1024 * 1024;
+  static constexpr int QS = HS == 512 && (!MANY || FMT == FMT_K8V4) ? 1 : 2;
+  static constexpr int MISC = 4 * 128 * 4 + 2 * 128 * 4 + 32 * 8 + 64;
+  static constexpr int RS0 = (231000 - QS * QREC - MISC) / STAGE;
+  static constexpr int RS = RS0 > 4 ? 4 : RS0;
+  static constexpr int OFF_RAW = QS * QREC;
+  static constexpr int OFF_KP = OFF_RAW + RS * STAGE;  // [4][128] float: key scale of the last tiles
+  static constexpr int OFF_RED = OFF_KP + 4 * 128 * 4;  // [2][128] float: the second half's sums
+  static constexpr int OFF_BAR = OFF_RED + 2 * 128 * 4;
+  static constexpr int OFF_TMEM = OFF_BAR + 32 * 8;
+  static constexpr int BYTES = OFF_TMEM + 64;  // the TMEM address, then where the share starts
+  static_assert(RS >= 2 && BYTES <= 232448, "shared memory");
+};
+
+enum { T_Q_FULL = 0, T_Q_EMPTY = 2, T_K_FULL = 4, T_K_FREE = 6, T_S_FULL = 8, T_S_FREE = 10, T_FINAL = 12 };
+
+// ---- the steps of a sequence: for each key group, the query tiles [first, end) with a row that sees one of its keys
+struct Steps {
+  int qlen, n, vis_base, group, window, ntq;
+};
+template <int NR>
+__device__ __forceinline__ Steps steps_of(const WeightParams& wp, int seq) {
+  const DecodeParams& p = wp.d;
+  Steps s;
+  s.qlen = p.cu_seqlens_q[seq + 1] - p.cu_seqlens_q[seq];
+  s.n = min(p.seqused_k[seq], wp.max_k);
+  s.vis_base = p.seqused_k[seq] - s.qlen + p.tokens_after;
+  s.group = p.group;
+  s.window = p.window;
+  s.ntq = (min(s.qlen, wp.max_q) * p.group + NR - 1) / NR;
+  if (s.qlen <= 0 || s.n < 0) s.n = s.ntq = 0;
+  return s;
+}
+template <int NR, int GK>
+__device__ __forceinline__ void tiles_seeing(const Steps& s, int g, int& first, int& end) {
+  const int lo = g * GK, hi = min(lo + GK, s.n) - 1;  // the group's keys
+  const int tok = max(0, lo - s.vis_base);
+  first = tok >= s.qlen ? s.ntq : static_cast<int>(static_cast<int64_t>(tok) * s.group / NR);
+  end = s.ntq;
+  if (s.window > 0) {
+    const int last = min(s.qlen - 1, hi + s.window - 1 - s.vis_base);
+    end = last < 0 ? first : max(first, static_cast<int>((static_cast<int64_t>(last + 1) * s.group - 1) / NR) + 1);
   }
-  const int rows = sp.qlen * p.group;
-  const float capl = p.softcap * LOG2E, cap_k = capl > 0.f ? 2.f * LOG2E / capl : 0.f;
-  float sum = 0.f;
-  for (int r0 = 0; r0 < rows; r0 += 8) {
-    __syncthreads();
-    for (int r = warp; r < 8 && r0 + r < rows; r += 4) {
-      const int tok = sp.q0 + (r0 + r) / p.group, qh = kvh * p.group + (r0 + r) % p.group;
-      const typename EL::T* src = reinterpret_cast<const typename EL::T*>(p.q) + tok * p.q_st + qh * p.q_sh + lane * E;
-      float x[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = EL::to_f(src[i]);
-      if (!p.q_rotated) {
-        apply_signs<E>(x, p.sign_bits, lane);
-        warp_wht<E>(x, lane);
+}
+template <int GK>
+__device__ __forceinline__ int groups_of(const Steps& s) { return (s.n + GK - 1) / GK; }
+// group from which the steps of a group are not all ntq any more (no window)
+template <int GK>
+__device__ __forceinline__ int full_groups(const Steps& s) {
+  return s.window > 0 ? 0 : max(0, min(groups_of<GK>(s), s.vis_base < 0 ? 0 : s.vis_base / GK + 1));
+}
+template <int NR, int GK>
+__device__ __forceinline__ int64_t count_steps(const Steps& s) {
+  const int full = full_groups<GK>(s), groups = groups_of<GK>(s);
+  int64_t t = static_cast<int64_t>(full) * s.ntq;
+  for (int g = full; g < groups; ++g) {
+    int a, b;
+    tiles_seeing<NR, GK>(s, g, a, b);
+    t += b - a;
+  }
+  return t;
+}
+
+// Walks a CTA's share: segments (sequence, KV head, group, query tiles [qa, qb)) in order. Every role runs its own.
+template <int NR, int GK>
+struct Walk {
+  int seq, kvh, g, qa, qb, first, end;  // the segment; all query tiles of its group
+  int qbase;                            // query tiles of the sequences before
+  int64_t left;                         // steps of the share not yet handed out
+  Steps s;
+
+  __device__ __forceinline__ bool next(const WeightParams& wp) {
+    if (left <= 0) return false;
+    for (;;) {
+      if (qb < end) {  // the group's tiles from qb on
+        qa = qb;
+        qb = static_cast<int>(min(static_cast<int64_t>(end), qa + left));
+        left -= qb - qa;
+        return true;
       }
+      if (++g >= groups_of<GK>(s)) {
+        g = 0;
+        if (++kvh == wp.d.nkv) {
+          kvh = 0;
+          do {
+            qbase += s.ntq;
+            s = steps_of<NR>(wp, ++seq);
+          } while (s.n == 0);
+        }
+      }
+      tiles_seeing<NR, GK>(s, g, first, end);
+      qb = first;
+    }
+  }
+};
+
+// What every CTA works out before it starts: the whole of the steps, its share and where that begins. In shared memory.
+struct ShareStart {
+  int64_t lo, hi;
+  int seq, kvh, g, q, qbase;
+};
+static_assert(sizeof(ShareStart) <= 48, "room beside the TMEM address");
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) qrow[r][lane * E + i] = x[i] * p.qk_scale;
-      if (lane == 0) row_lse[r] = wp.lse[static_cast<int64_t>(tok) * p.nq + qh];
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// The sequence that unit `at` lies in, units(b) units a sequence, and what comes before it of units and tiles(b).
+// scratch: 2 x 16 words of 64 bits. All `threads` threads call it and get the same answer in found[0..2].
+template <class U, class T>
+__device__ __forceinline__ void find_sequence(int num_seqs, int threads, int64_t at, U&& units, T&& tiles,
+                                              int64_t* scratch, int64_t* found) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
+  int64_t before_u = 0, before_t = 0;
+  for (int b0 = 0; b0 < num_seqs; b0 += threads) {
+    const int b = b0 + tid;
+    const int64_t u = b < num_seqs ? units(b) : 0, t = b < num_seqs ? tiles(b) : 0;
+    int64_t iu = u, it = t;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t ou = __shfl_up_sync(0xffffffffu, iu, d), ot = __shfl_up_sync(0xffffffffu, it, d);
+      if (lane >= d) {
+        iu += ou;
+        it += ot;
+      }
     }
     __syncthreads();
-    if (!valid) continue;
-    float s[8] = {};
-    for (int c = 0; c < HS; c += 2) {
-      float k0, k1;
-      if constexpr (FMT == FMT_INT4) {
-        const uint8_t b = cell[c / 2];
-        k0 = (b & 15) - zp;
-        k1 = (b >> 4) - zp;
+    if (lane == 31) {
+      scratch[warp] = iu;
+      scratch[16 + warp] = it;
+    }
+    __syncthreads();
+    int64_t bu = before_u, bt = before_t;
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) {
+        bu += scratch[w];
+        bt += scratch[16 + w];
+      }
+      before_u += scratch[w];
+      before_t += scratch[16 + w];
+    }
+    const int64_t start = bu + iu - u;
+    if (start <= at && at < start + u) {
+      found[0] = b;
+      found[1] = start;
+      found[2] = bt + it - t;
+    }
+    if (at < before_u) break;
+  }
+  __syncthreads();
+}
+
+template <int NR, int GK>
+__device__ __forceinline__ void find_start(const WeightParams& wp, int64_t* scratch, ShareStart* out) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const auto units = [&](int b) { return count_steps<NR, GK>(steps_of<NR>(wp, b)) * wp.d.nkv; };
+  int64_t total = 0;
+  for (int b = tid; b < wp.d.num_seqs; b += WT_THREADS) total += units(b);
+  total = warp_sum64(total);
+  if (lane == 0) scratch[warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < WT_THREADS / 32; ++w) total += scratch[w];
+  const int64_t share = (total + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * share, hi = min(lo + share, total);
+  int64_t* found = scratch + 32;
+  if (lo < hi)
+    find_sequence(wp.d.num_seqs, WT_THREADS, lo, units, [&](int b) { return steps_of<NR>(wp, b).ntq; }, scratch,
+                  found);
+  if (tid == 0) {
+    out->lo = lo;
+    out->hi = max(lo, hi);
+    if (lo < hi) {
+      out->seq = static_cast<int>(found[0]);
+      out->qbase = static_cast<int>(found[2]);
+      const Steps s = steps_of<NR>(wp, out->seq);
+      const int64_t each = count_steps<NR, GK>(s);
+      out->kvh = static_cast<int>((lo - found[1]) / each);
+      int64_t u = (lo - found[1]) % each;
+      const int full = full_groups<GK>(s);
+      int g, a, b;
+      if (u < static_cast<int64_t>(full) * s.ntq) {
+        g = static_cast<int>(u / s.ntq);
+        u -= static_cast<int64_t>(g) * s.ntq;
+        a = 0;
       } else {
-        k0 = static_cast<int8_t>(cell[c]);
-        k1 = static_cast<int8_t>(cell[c + 1]);
+        u -= static_cast<int64_t>(full) * s.ntq;
+        for (g = full;; ++g) {
+          tiles_seeing<NR, GK>(s, g, a, b);
+          if (u < b - a) break;
+          u -= b - a;
+        }
       }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) s[r] = fmaf(k1, qrow[r][c + 1], fmaf(k0, qrow[r][c], s[r]));
-    }
-    for (int r = 0; r < 8 && r0 + r < rows; ++r) {
-      const int vis = sp.vis_base + (r0 + r) / p.group;
-      float t = s[r] * ks;
-      if (capl > 0.f) t = softcap_log2(t, capl, cap_k);
-      if (key <= vis && (p.window <= 0 || key > vis - p.window) && row_lse[r] != -INFINITY)
-        sum += exp2f(t - row_lse[r]);
+      out->g = g;
+      out->q = a + static_cast<int>(u);
     }
   }
-  if (!valid) return;
-  if (key >= sp.vis_base) wp.weights[at] = sum;  // the call's own tokens: no earlier weight
-  else atomicAdd(wp.weights + at, sum);          // a page may be shared by sequences of the call
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------------------- K4q
+// One CTA per query tile: NR rows of a (sequence, KV head), rotated and scaled by a power of two common to the tile
+// (|q| < 2^14 at its largest finite value: a row far smaller keeps the tile's absolute accuracy, which is what an
+// exponent needs), as two fp16 terms in the operand's layout; -lse (a row without keys, and a padding row: -inf) and
+// the first and last key of each row.
+template <int FMT, int DT, int HS, int NR, bool MANY>
+__global__ void __launch_bounds__(256) weights_qprep_kernel(const WeightParams wp) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  using W = WT<FMT, HS, NR, 1, MANY>;
+  using EL = Elem<DT>;
+  constexpr int E = HS / 32, RW = NR / 8;  // channels a lane, rows a warp
+  const DecodeParams& p = wp.d;
+  __shared__ int64_t scratch[36];
+  __shared__ float wmax[8];
+  __shared__ int wvis[8], wlo[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y;
+  int seq = blockIdx.x, qt = 0;
+  if constexpr (MANY) {
+    if (p.num_seqs == 1) {
+      seq = 0;
+      qt = blockIdx.x;
+    } else {
+      if (tid == 0) scratch[32] = -1;
+      const auto tiles = [&](int b) { return static_cast<int64_t>(steps_of<NR>(wp, b).ntq); };
+      find_sequence(p.num_seqs, 256, blockIdx.x, tiles, tiles, scratch, scratch + 32);
+      if (scratch[32] < 0) return;
+      seq = static_cast<int>(scratch[32]);
+      qt = static_cast<int>(blockIdx.x - scratch[33]);
+    }
+  }
+  const Steps s = steps_of<NR>(wp, seq);
+  if (qt >= s.ntq) return;
+  // the record's place: the sequences' tiles in a row (one place each where none has more), KV heads inside
+  uint8_t* rec = wp.qrec + (static_cast<int64_t>(blockIdx.x) * p.nkv + kvh) * W::QREC;
+  const int q0 = p.cu_seqlens_q[seq], rows = s.qlen * p.group;
+  float x[RW][E];
+  float am = 0.f;
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int r = qt * NR + warp * RW + i;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+    if (r < rows) {
+      const int tok = q0 + r / p.group, qh = kvh * p.group + r % p.group;
+      const typename EL::T* src = reinterpret_cast<const typename EL::T*>(p.q) + tok * p.q_st + qh * p.q_sh + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = EL::to_f(src[e]);
+      if (!p.q_rotated) {
+        apply_signs<E>(x[i], p.sign_bits, lane);
+        warp_wht<E>(x[i], lane);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) am = fmaxf(am, fabsf(x[i][e]) < INFINITY ? fabsf(x[i][e]) : 0.f);
+    }
+  }
+  am = warp_max(am);
+  int vis_min = INT_MAX, lo_max = INT_MIN;
+  if (lane < RW) {  // this lane's row of the warp: its bounds and -lse
+    const int rt = warp * RW + lane, r = qt * NR + rt;
+    float nl = -INFINITY;
+    int vis = INT_MAX, lo = INT_MIN;
+    if (r < rows) {
+      const int tok = r / p.group;
+      const float l = wp.lse[static_cast<int64_t>(q0 + tok) * p.nq + kvh * p.group + r % p.group];
+      if (l != -INFINITY) nl = -l;
+      vis = s.vis_base + tok;
+      if (p.window > 0) lo = vis - p.window + 1;
+      vis_min = vis;
+      lo_max = lo;
+    }
+    reinterpret_cast<float*>(rec + W::ROWS)[rt] = nl;
+    reinterpret_cast<int*>(rec + W::ROWS)[NR + rt] = vis;
+    reinterpret_cast<int*>(rec + W::ROWS)[2 * NR + rt] = lo;
+  }
+  vis_min = __reduce_min_sync(0xffffffffu, vis_min);
+  lo_max = __reduce_max_sync(0xffffffffu, lo_max);
+  if (lane == 0) {
+    wmax[warp] = am;
+    wvis[warp] = vis_min;
+    wlo[warp] = lo_max;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    am = fmaxf(am, wmax[w]);
+    vis_min = min(vis_min, wvis[w]);
+    lo_max = max(lo_max, wlo[w]);
+  }
+  int ex = 0;
+  if (am > 0.f) {
+    frexpf(am, &ex);
+    ex = 14 - ex;
+  }
+  if (tid == 0)
+    *reinterpret_cast<float4*>(rec + W::HEAD) =
+        make_float4(ldexpf(p.qk_scale, -ex), __int_as_float(vis_min), __int_as_float(lo_max), 0.f);
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int rt = warp * RW + i;
+    __half hi[E], lo[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float y = ldexpf(x[i][e], ex);
+      hi[e] = __float2half_rn(y);
+      lo[e] = __float2half_rn(y - __half2float(hi[e]));
+    }
+    // byte of channel pair k, k + 1 of a term: atom k / 64, row rt, swizzled 16-byte chunk
+    const auto put = [&](int term, int chunk, const uint4& v) {
+      *reinterpret_cast<uint4*>(rec + term * W::TERM + (chunk >> 3) * W::ATOM + sw128_off(rt, chunk & 7)) = v;
+    };
+    const auto two = [](__half a, __half b) {
+      return static_cast<uint32_t>(__half_as_ushort(a)) | (static_cast<uint32_t>(__half_as_ushort(b)) << 16);
+    };
+    if constexpr (E == 4) {
+      // two lanes hold a chunk's eight channels: the even lane writes the first term's, the odd lane the second's
+      const bool odd = lane & 1;
+      const uint32_t a0 = odd ? two(lo[0], lo[1]) : two(hi[0], hi[1]), a1 = odd ? two(lo[2], lo[3]) : two(hi[2], hi[3]);
+      const uint32_t g0 = odd ? two(hi[0], hi[1]) : two(lo[0], lo[1]), g1 = odd ? two(hi[2], hi[3]) : two(lo[2], lo[3]);
+      const uint32_t b0 = __shfl_xor_sync(0xffffffffu, g0, 1), b1 = __shfl_xor_sync(0xffffffffu, g1, 1);
+      const uint32_t e0 = odd ? b0 : a0, e1 = odd ? b1 : a1, o0 = odd ? a0 : b0, o1 = odd ? a1 : b1;
+      if constexpr (FMT == FMT_INT4)  // k order: channels 0 4 1 5 2 6 3 7
+        put(odd, lane >> 1, make_uint4(prmt(e0, o0, 0x5410u), prmt(e0, o0, 0x7632u), prmt(e1, o1, 0x5410u),
+                                       prmt(e1, o1, 0x7632u)));
+      else put(odd, lane >> 1, make_uint4(e0, e1, o0, o1));
+    } else {
+#pragma unroll
+      for (int c = 0; c < E / 8; ++c) {
+#pragma unroll
+        for (int term = 0; term < 2; ++term) {
+          const __half* h = (term ? lo : hi) + 8 * c;
+          if constexpr (FMT == FMT_INT4)
+            put(term, lane * (E / 8) + c, make_uint4(two(h[0], h[4]), two(h[1], h[5]), two(h[2], h[6]), two(h[3], h[7])));
+          else
+            put(term, lane * (E / 8) + c, make_uint4(two(h[0], h[1]), two(h[2], h[3]), two(h[4], h[5]), two(h[6], h[7])));
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// 32 TMEM columns (64 channels) of a key's exact codes from 32 (int4) or 64 (k8v4) bytes
+template <int FMT>
+__device__ __forceinline__ void key_columns(const uint8_t* codes, uint32_t lo_bias, uint32_t hi_bias, uint32_t (&a)[32]) {
+  if constexpr (FMT == FMT_INT4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint2 w2 = *reinterpret_cast<const uint2*>(codes + 8 * k);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t w = e ? w2.y : w2.x, w8 = w >> 8;
+        const int j = 8 * k + 4 * e;
+        // 1024 + u minus 1024 + zp; (1024 + 16 u) / 16 minus 64 + zp: channels 8 w + {0, 4}, {1, 5}, {2, 6}, {3, 7}
+        a[j] = hsub2_u32(lop3_and_or(w, 0x000F000Fu, 0x64006400u), lo_bias);
+        a[j + 1] = hfma2_u32(lop3_and_or(w, 0x00F000F0u, 0x64006400u), 0x2C002C00u, hi_bias);
+        a[j + 2] = hsub2_u32(lop3_and_or(w8, 0x000F000Fu, 0x64006400u), lo_bias);
+        a[j + 3] = hfma2_u32(lop3_and_or(w8, 0x00F000F0u, 0x64006400u), 0x2C002C00u, hi_bias);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint2 w2 = *reinterpret_cast<const uint2*>(codes + 8 * k);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t x = (e ? w2.y : w2.x) ^ 0x80808080u;  // 1024 + (c + 128) minus 1152
+        a[4 * k + 2 * e] = hsub2_u32(prmt(x, 0x64646464u, 0x4140u), 0x64806480u);
+        a[4 * k + 2 * e + 1] = hsub2_u32(prmt(x, 0x64646464u, 0x4342u), 0x64806480u);
+      }
+    }
+  }
+}
+
+// The call's own tokens have no earlier weight; a page of the others may be shared by sequences of the call.
+__device__ __forceinline__ void add_weight(const WeightParams& wp, int seq, int kvh, int key, int vis_base, float w) {
+  const DecodeParams& p = wp.d;
+  const int b = key / p.block_size;
+  float* at = wp.weights + p.block_table[seq * p.bt_stride + b] * wp.w_block +
+              static_cast<int64_t>(key - b * p.block_size) * wp.w_slot + kvh * wp.w_head;
+  if (key >= vis_base) *at = w;
+  else atomicAdd(at, w);
+}
+
+// ---------------------------------------------------------------------------------------------------- K4
+template <int FMT, int HS, int NR, int KT, bool MANY, bool CAP>
+__global__ void __launch_bounds__(WT_THREADS, 1) weights_kernel(const WeightParams wp) {
+  using W = WT<FMT, HS, NR, KT, MANY>;
+  using CL = typename W::CL;
+  constexpr int GK = WT_KEYS * KT, SLOTS = W::SLOTS, RS = W::RS, QS = W::QS;
+  const DecodeParams& p = wp.d;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + W::OFF_TMEM);
+  // (no static shared memory: the operand's swizzle wants the dynamic part at a multiple of 1024 bytes)
+  ShareStart& start = *reinterpret_cast<ShareStart*>(smem + W::OFF_TMEM + 16);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[T_Q_FULL + i], 1);
+      mbar_init(&bars[T_Q_EMPTY + i], 1 + 8);
+      mbar_init(&bars[T_K_FULL + i], 4);
+      mbar_init(&bars[T_K_FREE + i], 1);
+      mbar_init(&bars[T_S_FULL + i], 1);
+      mbar_init(&bars[T_S_FREE + i], 8);
+    }
+    mbar_init(&bars[T_FINAL], 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, W::COLS);
+    tmem_relinquish();
+  }
+  find_start<NR, GK>(wp, reinterpret_cast<int64_t*>(smem + W::OFF_RAW), &start);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Walk<NR, GK> walk;
+  walk.left = start.hi - start.lo;
+  if (walk.left > 0) {
+    walk.seq = start.seq;
+    walk.kvh = start.kvh;
+    walk.g = start.g;
+    walk.qbase = start.qbase;
+    walk.s = steps_of<NR>(wp, start.seq);
+    tiles_seeing<NR, GK>(walk.s, walk.g, walk.first, walk.end);
+    walk.qb = start.q;
+  }
+  const auto tiles_in = [&]() {  // key tiles of the group that hold keys
+    return min(KT, (walk.s.n - walk.g * GK + WT_KEYS - 1) / WT_KEYS);
+  };
+  const auto tile_id = [&](int qt) { return static_cast<int64_t>(MANY ? walk.qbase + qt : walk.seq) * p.nkv + walk.kvh; };
+  bool ok = true;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ query tiles
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // K4q's records
+    int64_t cur = -1;
+    int loads = 0;
+    while (ok && walk.next(wp)) {
+      for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
+        const int64_t id = tile_id(qt);
+        if (id == cur) continue;
+        cur = id;
+        const int st = loads % QS;
+        if (loads >= QS) ok = !__any_sync(0xffffffffu, !mbar_wait_bounded(&bars[T_Q_EMPTY + st], (loads / QS - 1) & 1));
+        if (ok && lane == 0) {
+          mbar_arrive_expect_tx(&bars[T_Q_FULL + st], W::QREC);
+          bulk_g2s(smem + st * W::QREC, wp.qrec + id * W::QREC, W::QREC, &bars[T_Q_FULL + st]);
+        }
+        __syncwarp();
+        ++loads;
+      }
+    }
+    // the copies in flight land before the CTA's shared memory can go away
+    for (int k = max(0, loads - QS); k < loads; ++k) mbar_wait_bounded(&bars[T_Q_FULL + k % QS], (k / QS) & 1);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMAs
+    constexpr uint32_t ID = f16_idesc(128, NR, false);
+    int64_t cur = -1;
+    int loads = 0, jobs = 0, tiles = 0;  // query tiles seen, S buffers filled, key tiles before this group
+    const auto wait = [&](int bar, uint32_t parity) {
+      if (ok) ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[bar], parity));
+    };
+    while (ok && walk.next(wp)) {
+      const int kt = tiles_in();
+      for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
+        const int64_t id = tile_id(qt);
+        if (id != cur) {
+          if (loads > 0 && elect_one()) umma_commit(&bars[T_Q_EMPTY + (loads - 1) % QS]);
+          __syncwarp();
+          cur = id;
+          wait(T_Q_FULL + loads % QS, (loads / QS) & 1);
+          ++loads;
+        }
+        const uint64_t qd = sw128_desc(smem_u32(smem + ((loads - 1) % QS) * W::QREC), 16, 1024);
+        for (int t = 0; t < kt && ok; ++t, ++jobs) {
+          const int tile = tiles + t, sl = tile % SLOTS, b = jobs & 1;
+          if (qt == walk.qa) wait(T_K_FULL + sl, (tile / SLOTS) & 1);
+          if (jobs >= 2) wait(T_S_FREE + b, (jobs / 2 - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t ak = tmem + sl * W::ACOLS, sd = tmem + W::S + b * NR;
+#pragma unroll
+            for (int term = 0; term < 2; ++term)
+#pragma unroll
+              for (int c = 0; c < HS / 16; ++c)
+                umma_f16_ts(sd, ak + 8 * c,
+                            qd + static_cast<uint64_t>((term * W::TERM + (c >> 2) * W::ATOM + (c & 3) * 32) >> 4), ID,
+                            (term | c) ? 1u : 0u);
+            umma_commit(&bars[T_S_FULL + b]);
+            if (qt == walk.qb - 1) umma_commit(&bars[T_K_FREE + sl]);
+          }
+          __syncwarp();
+        }
+      }
+      tiles += kt;
+    }
+    if (elect_one()) umma_commit(&bars[T_FINAL]);
+    __syncwarp();
+    mbar_wait_spin(&bars[T_FINAL], 0);  // every MMA has completed before TMEM goes
+  } else if (warp < 6) {
+    // ------------------------------------------------------------------ keys (thread = key = TMEM lane)
+    const int ct = tid - 64, quarter = warp & 3, kl = 32 * quarter + lane;
+    float* kp = reinterpret_cast<float*>(smem + W::OFF_KP);
+    // the raw stages are filled one walk ahead of the conversion
+    Walk<NR, GK> ahead = walk;
+    int at = 0, kt_ahead = 0;
+    const uint8_t* run = nullptr;  // lanes 0-7: the tile's 16-cell runs
+    const auto issue = [&](int tile) {
+      if (at == kt_ahead) {
+        at = 0;
+        kt_ahead = ahead.next(wp) ? min(KT, (ahead.s.n - ahead.g * GK + WT_KEYS - 1) / WT_KEYS) : 0;
+      }
+      if (at < kt_ahead) {
+        const int k0 = ahead.g * GK + at * WT_KEYS, mine = k0 + 16 * (lane & 7);
+        run = nullptr;
+        if (mine < ahead.s.n) {
+          const int32_t page = p.block_table[ahead.seq * p.bt_stride + mine / p.block_size];
+          run = p.cache + static_cast<int64_t>(page) * p.block_stride +
+                static_cast<int64_t>(ahead.kvh) * p.head_stride +
+                static_cast<int64_t>(mine % p.block_size) * CL::BYTES;
+        }
+        uint8_t* dst = smem + W::OFF_RAW + (tile % RS) * W::STAGE;
+#pragma unroll 4
+        for (int e = 0; e < W::PIECES; ++e) {
+          const int idx = e * 128 + ct, key = idx / W::PIECES, piece = idx - key * W::PIECES;
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(run), key >> 4));
+          if (k0 + key < ahead.s.n) cp_async8(dst + idx * 8, src + (key & 15) * CL::BYTES + piece * 8);
+        }
+        ++at;
+      }
+      cp_async_commit();
+    };
+    int tile = 0;
+    bool leave = false;  // set for all four warps at once
+#pragma unroll
+    for (int i = 0; i < RS - 1; ++i) issue(i);
+    while (!leave && walk.next(wp)) {
+      const int kt = tiles_in();
+      for (int t = 0; t < kt; ++t, ++tile) {
+        cp_async_wait<RS - 2>();
+        leave = named_bar_or(1, 128, !ok);
+        if (leave) break;
+        issue(tile + RS - 1);  // into the stage that every thread has left
+        const int sl = tile % SLOTS;
+        if (tile >= SLOTS)
+          ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_K_FREE + sl], (tile / SLOTS - 1) & 1));
+        if (!ok) continue;
+        tc_fence_after();
+        const uint8_t* raw = smem + W::OFF_RAW + (tile % RS) * W::STAGE + kl * W::KEY;
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(raw + CL::KB);
+        const uint32_t zp = FMT == FMT_INT4 ? word & 0xFu : 0u;
+        const uint32_t lo1 = 0x6400u | zp, hi1 = 0xD400u | (zp << 4);  // 1024 + zp, -(64 + zp)
+        const uint32_t ta = tmem + sl * W::ACOLS + (static_cast<uint32_t>(32 * quarter) << 16);
+#pragma unroll 1
+        for (int c = 0; c < HS / 64; ++c) {
+          uint32_t a[32];
+          key_columns<FMT>(raw + c * (CL::KB / (HS / 64)), lo1 | (lo1 << 16), hi1 | (hi1 << 16), a);
+          tmem_st32u(ta + 32 * c, a);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        const bool valid = walk.g * GK + t * WT_KEYS + kl < walk.s.n;
+        kp[(tile & 3) * 128 + kl] = !valid ? 0.f : __uint_as_float(FMT == FMT_INT4 ? word & 0xFFFFFFF0u : word);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[T_K_FULL + sl]);
+      }
+    }
+    cp_async_wait<0>();
+  } else {
+    // ------------------------------------------------------------------ weights (thread = key, half of the columns)
+    constexpr int NH = NR / 2, CH = NH < 16 ? NH : 16;  // columns a thread, and at a time
+    const int quarter = warp & 3, half = (warp - 6) >> 2, kl = 32 * quarter + lane;
+    const uint32_t ta = tmem + W::S + half * NH + (static_cast<uint32_t>(32 * quarter) << 16);
+    const float* kp = reinterpret_cast<const float*>(smem + W::OFF_KP);
+    float* red = reinterpret_cast<float*>(smem + W::OFF_RED);
+    const float capl = CAP ? p.softcap * LOG2E : 0.f, cap_k = CAP ? 2.f * LOG2E / capl : 0.f;
+    int64_t cur = -1;
+    int loads = 0, jobs = 0, tiles = 0, sums = 0;
+    int4 rec_head = make_int4(0, 0, 0, 0), rec_tail = make_int4(0, 0, 0, 0);
+    while (walk.next(wp)) {
+      const int kt = tiles_in();
+      float ks[KT];
+      float2 sum[KT];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) sum[t] = make_float2(0.f, 0.f);
+      for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
+        const int64_t id = tile_id(qt);
+        if (id != cur) {
+          if (loads > 0 && lane == 0) mbar_arrive(&bars[T_Q_EMPTY + (loads - 1) % QS]);
+          cur = id;
+          ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_Q_FULL + loads % QS], (loads / QS) & 1));
+          ++loads;
+        }
+        const uint8_t* rec = smem + ((loads - 1) % QS) * W::QREC;
+        const float4 hd = *reinterpret_cast<const float4*>(rec + W::HEAD);
+        const float* nl = reinterpret_cast<const float*>(rec + W::ROWS) + half * NH;
+        const int* vis = reinterpret_cast<const int*>(rec + W::ROWS) + NR + half * NH;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          if (t >= kt || !ok) break;
+          const int b = jobs & 1, k0 = walk.g * GK + t * WT_KEYS;
+          ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_S_FULL + b], (jobs / 2) & 1));
+          ++jobs;
+          if (!ok) break;
+          tc_fence_after();
+          if (qt == walk.qa) ks[t] = kp[((tiles + t) & 3) * 128 + kl];
+          const float k1 = ks[t] * hd.x;
+          const bool masked = k0 + WT_KEYS - 1 > __float_as_int(hd.y) || k0 < __float_as_int(hd.z);
+#pragma unroll
+          for (int c0 = 0; c0 < NH; c0 += CH) {
+            float sc[CH];
+            tmem_ld_cols<CH>(ta + b * NR + c0, sc);
+            if (c0 + CH == NH) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars[T_S_FREE + b]);
+            }
+#pragma unroll
+            for (int c = 0; c < CH; c += 4) {
+              const float4 l4 = *reinterpret_cast<const float4*>(nl + c0 + c);
+              float2 x[2];
+              if constexpr (!CAP) {
+                x[0] = __ffma2_rn(make_float2(sc[c], sc[c + 1]), make_float2(k1, k1), make_float2(l4.x, l4.y));
+                x[1] = __ffma2_rn(make_float2(sc[c + 2], sc[c + 3]), make_float2(k1, k1), make_float2(l4.z, l4.w));
+              } else {
+                x[0] = make_float2(softcap_log2(sc[c] * k1, capl, cap_k) + l4.x,
+                                   softcap_log2(sc[c + 1] * k1, capl, cap_k) + l4.y);
+                x[1] = make_float2(softcap_log2(sc[c + 2] * k1, capl, cap_k) + l4.z,
+                                   softcap_log2(sc[c + 3] * k1, capl, cap_k) + l4.w);
+              }
+              if (masked) {
+                const int key = k0 + kl;
+                const int4 v = *reinterpret_cast<const int4*>(vis + c0 + c);
+                const int4 f = *reinterpret_cast<const int4*>(vis + NR + c0 + c);
+                if (key > v.x || key < f.x) x[0].x = -INFINITY;
+                if (key > v.y || key < f.y) x[0].y = -INFINITY;
+                if (key > v.z || key < f.z) x[1].x = -INFINITY;
+                if (key > v.w || key < f.w) x[1].y = -INFINITY;
+              }
+              sum[t] = __fadd2_rn(sum[t], make_float2(fast_exp2(x[0].x), fast_exp2(x[0].y)));
+              sum[t] = __fadd2_rn(sum[t], make_float2(fast_exp2(x[1].x), fast_exp2(x[1].y)));
+            }
+          }
+        }
+      }
+      // the halves' sums meet; whole groups go to the weights, parts of one to the workspace
+      const bool head = walk.qa > walk.first, tail = walk.qb < walk.end;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        if (t >= kt) break;
+        float* r = red + (sums++ & 1) * 128;
+        if (half == 1) r[kl] = sum[t].x + sum[t].y;
+        if (named_bar_or(2, 256, !ok)) {
+          ok = false;
+          break;
+        }
+        const int key = walk.g * GK + t * WT_KEYS + kl;
+        if (half == 0 && key < walk.s.n) {
+          const float w = sum[t].x + sum[t].y + r[kl];
+          if (head || tail)
+            wp.part[(static_cast<int64_t>(blockIdx.x) * 2 + (head ? 0 : 1)) * 256 + t * WT_KEYS + kl] = w;
+          else add_weight(wp, walk.seq, walk.kvh, key, walk.s.vis_base, w);
+        }
+      }
+      if (!ok) break;
+      if (head) rec_head = make_int4(1, tail, 0, 0);
+      else if (tail) rec_tail = make_int4(1, walk.seq, walk.kvh, walk.g);
+      tiles += kt;
+    }
+    if (MANY && warp == 6 && lane == 0) {
+      wp.records[2 * blockIdx.x] = rec_head;
+      wp.records[2 * blockIdx.x + 1] = rec_tail;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, W::COLS);
+}
+
+// ---------------------------------------------------------------------------------------------------- K4f
+// One CTA per CTA of K4 that began a group it did not finish: the parts of the group, in order.
+template <int GK>
+__global__ void __launch_bounds__(GK) weights_fold_kernel(const WeightParams wp) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 rec = wp.records[2 * blockIdx.x + 1];
+  if (!rec.x) return;
+  float w = wp.part[(static_cast<int64_t>(blockIdx.x) * 2 + 1) * 256 + threadIdx.x];
+  for (int c = blockIdx.x + 1; c < gridDim.x; ++c) {
+    const int4 r = wp.records[2 * c];
+    if (!r.x) break;
+    w += wp.part[static_cast<int64_t>(c) * 512 + threadIdx.x];
+    if (!r.y) break;
+  }
+  const Steps s = steps_of<16>(wp, rec.y);
+  const int key = rec.w * GK + threadIdx.x;
+  if (key < s.n) add_weight(wp, rec.y, rec.z, key, s.vis_base, w);
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+static cudaLaunchConfig_t wt_config(const dim3& grid, int threads, int smem, cudaStream_t st, cudaLaunchAttribute* pdl) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  pdl->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl->val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+template <int FMT, int DT, int HS, int NR, int KT, bool MANY, bool CAP>
+static int launch_weights_t(const WeightParams& wp, int64_t tiles, int ctas, cudaStream_t st) {
+  using W = WT<FMT, HS, NR, KT, MANY>;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(weights_kernel<FMT, HS, NR, KT, MANY, CAP>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, W::BYTES);
+    if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "attention weights attribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  weights_qprep_kernel<FMT, DT, HS, NR, MANY><<<dim3(static_cast<unsigned>(tiles), wp.d.nkv), 256, 0, st>>>(wp);
+  int rc = check_launch("attention weights q prep");
+  if (rc) return rc;
+  cudaLaunchAttribute pdl[1];
+  cudaLaunchConfig_t cfg = wt_config(dim3(ctas), WT_THREADS, W::BYTES, st, pdl);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, weights_kernel<FMT, HS, NR, KT, MANY, CAP>, wp);
+  if (e == cudaSuccess && MANY) {
+    cfg = wt_config(dim3(ctas), WT_KEYS * KT, 0, st, pdl);
+    e = cudaLaunchKernelEx(&cfg, weights_fold_kernel<WT_KEYS * KT>, wp);
+  }
+  if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "attention weights launch: %s", cudaGetErrorString(e));
+  return QP_OK;
+}
+
+// rows of a query tile: all of a sequence's where they are few, else what keeps a tile at 64 KB or two S^T buffers
+// beside two key tiles in TMEM
+static int wt_tile_rows(int rows, int head_size) {
+  if (rows <= 16) return 16;
+  if (rows <= WT_SMALL_ROWS || head_size == 512) return 32;
+  return 64;
+}
+// query tiles (of one KV head) that a call may have at most
+static int64_t wt_tiles(int64_t num_q_tokens, int num_seqs, int max_seqlen_q, int group, int head_size) {
+  const int64_t rows = static_cast<int64_t>(max_seqlen_q) * group;
+  if (rows <= WT_SMALL_ROWS) return num_seqs;
+  const int nr = wt_tile_rows(WT_SMALL_ROWS + 1, head_size);
+  return std::min(num_q_tokens * group / nr + num_seqs, num_seqs * ((rows + nr - 1) / nr));
+}
+
+template <int FMT, int DT, int HS, bool CAP>
+static int launch_weights_hs(const WeightParams& wp, int64_t rows, int64_t tiles, int ctas, cudaStream_t st) {
+  if (rows <= 16) return launch_weights_t<FMT, DT, HS, 16, 1, false, CAP>(wp, tiles, ctas, st);
+  if (rows <= WT_SMALL_ROWS) return launch_weights_t<FMT, DT, HS, 32, 1, false, CAP>(wp, tiles, ctas, st);
+  if constexpr (HS == 512) return launch_weights_t<FMT, DT, HS, 32, 1, true, CAP>(wp, tiles, ctas, st);
+  else return launch_weights_t<FMT, DT, HS, 64, 2, true, CAP>(wp, tiles, ctas, st);
+}
+
+template <int FMT, int DT, bool CAP>
+static int launch_weights_cap(const WeightParams& wp, int head_size, int64_t rows, int64_t tiles, int ctas,
+                              cudaStream_t st) {
+  if (head_size == 128) return launch_weights_hs<FMT, DT, 128, CAP>(wp, rows, tiles, ctas, st);
+  if (head_size == 256) return launch_weights_hs<FMT, DT, 256, CAP>(wp, rows, tiles, ctas, st);
+  return launch_weights_hs<FMT, DT, 512, CAP>(wp, rows, tiles, ctas, st);
 }
 
 template <int FMT, int DT>
-static int launch_weights(const WeightParams& wp, const dim3& grid, cudaStream_t st) {
-  switch (wp.head_size) {
-    case 128: weights_kernel<FMT, DT, 128><<<grid, 128, 0, st>>>(wp); break;
-    case 256: weights_kernel<FMT, DT, 256><<<grid, 128, 0, st>>>(wp); break;
-    default: weights_kernel<FMT, DT, 512><<<grid, 128, 0, st>>>(wp); break;
-  }
-  return check_launch("attention weights");
+static int launch_weights(const WeightParams& wp, int head_size, int64_t rows, int64_t tiles, int ctas,
+                          cudaStream_t st) {
+  return wp.d.softcap > 0.f ? launch_weights_cap<FMT, DT, true>(wp, head_size, rows, tiles, ctas, st)
+                            : launch_weights_cap<FMT, DT, false>(wp, head_size, rows, tiles, ctas, st);
+}
+
+static int64_t wt_record_bytes(int rows, int head_size) {
+  return (rows * head_size * 4ll + 12 * rows + 16 + 1023) / 1024 * 1024;
 }
 
 }  // namespace qp
 
 using namespace qp;
 
-extern "C" int64_t qp_attn_weights_workspace_bytes(int64_t num_q_tokens, int num_seqs, int num_q_heads,
-                                                   int num_kv_heads, int head_size) {
-  return 256;
+// [per CTA: two sums of 256 keys, fp32][per CTA: two records of 16 bytes][prepared query tiles]
+static int64_t wt_tiles_offset(int ctas) { return (static_cast<int64_t>(ctas) * (2 * 256 * 4 + 32) + 1023) / 1024 * 1024; }
+
+extern "C" int64_t qp_attn_weights_workspace_bytes(int64_t num_q_tokens, int num_seqs, int max_seqlen_q,
+                                                   int num_q_heads, int num_kv_heads, int head_size) {
+  if (num_q_tokens <= 0 || num_seqs <= 0 || max_seqlen_q <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads)
+    return 1024;
+  const int group = num_q_heads / num_kv_heads;
+  const int64_t rows = std::min<int64_t>(static_cast<int64_t>(max_seqlen_q) * group, 1 << 20);
+  return wt_tiles_offset(device_sm_count()) +
+         wt_tiles(num_q_tokens, num_seqs, max_seqlen_q, group, head_size) * num_kv_heads *
+             wt_record_bytes(wt_tile_rows(static_cast<int>(rows), head_size), head_size);
 }
 
 extern "C" int qp_accumulate_attn_weights(int fmt, int dtype, const void* q, int64_t q_stride_token,
@@ -138,10 +905,13 @@ extern "C" int qp_accumulate_attn_weights(int fmt, int dtype, const void* q, int
   if (sliding_window < 0) return set_error(QP_ERR_INVALID, "attention weights: sliding_window %d", sliding_window);
   if (!(softcap >= 0.f) || isinf(softcap)) return set_error(QP_ERR_INVALID, "attention weights: softcap %g", softcap);
   if (num_seqs == 0 || num_q_tokens == 0 || max_seqlen_q == 0 || max_seqlen_k == 0) return QP_OK;
-  if (num_seqs > 65535 || num_kv_heads > 65535) return set_error(QP_ERR_UNSUPPORTED, "attention weights: grid too large");
+  if (num_seqs > 65535 || num_kv_heads > 65535 ||
+      static_cast<int64_t>(max_seqlen_q) * (num_q_heads / num_kv_heads) > 0x3fffffff)
+    return set_error(QP_ERR_UNSUPPORTED, "attention weights: grid too large");
   if (!q || !cu_seqlens_q || !seqused_k || !block_table || !cache || !rht_sign_bits || !lse || !weights || !workspace)
     return set_error(QP_ERR_INVALID, "attention weights: null pointer");
-  const int64_t need = qp_attn_weights_workspace_bytes(num_q_tokens, num_seqs, num_q_heads, num_kv_heads, head_size);
+  const int64_t need = qp_attn_weights_workspace_bytes(num_q_tokens, num_seqs, max_seqlen_q, num_q_heads,
+                                                       num_kv_heads, head_size);
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)
     return set_error(QP_ERR_WORKSPACE, "attention weights: workspace of %lld bytes < %lld", (long long)workspace_bytes,
                      (long long)need);
@@ -175,11 +945,23 @@ extern "C" int qp_accumulate_attn_weights(int fmt, int dtype, const void* q, int
   wp.w_block = weights_stride_block;
   wp.w_slot = weights_stride_slot;
   wp.w_head = weights_stride_head;
-  wp.head_size = head_size;
-  const dim3 grid(static_cast<unsigned>((max_seqlen_k + 127) / 128), static_cast<unsigned>(num_kv_heads),
-                  static_cast<unsigned>(num_seqs));
+  wp.max_q = max_seqlen_q;
+  wp.max_k = max_seqlen_k;
+  const int sms = device_sm_count();
+  wp.part = static_cast<float*>(workspace);
+  wp.records = reinterpret_cast<int4*>(wp.part + static_cast<int64_t>(sms) * 2 * 256);
+  wp.qrec = static_cast<uint8_t*>(workspace) + wt_tiles_offset(sms);
+  const int64_t rows = static_cast<int64_t>(max_seqlen_q) * dp.group;
+  const int64_t tiles = wt_tiles(num_q_tokens, num_seqs, max_seqlen_q, dp.group, head_size);
+  if (tiles > 0x7fffffff) return set_error(QP_ERR_UNSUPPORTED, "attention weights: too many query rows");
+  // no more CTAs than there may be steps
+  const int64_t steps = static_cast<int64_t>(num_kv_heads) * ((max_seqlen_k + WT_KEYS - 1) / WT_KEYS) *
+                        std::max<int64_t>(tiles, num_seqs);
+  const int ctas = static_cast<int>(std::min<int64_t>(sms, steps));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (fmt == FMT_INT4)
-    return dtype == DT_BF16 ? launch_weights<FMT_INT4, DT_BF16>(wp, grid, st) : launch_weights<FMT_INT4, DT_F16>(wp, grid, st);
-  return dtype == DT_BF16 ? launch_weights<FMT_K8V4, DT_BF16>(wp, grid, st) : launch_weights<FMT_K8V4, DT_F16>(wp, grid, st);
+    return dtype == DT_BF16 ? launch_weights<FMT_INT4, DT_BF16>(wp, head_size, rows, tiles, ctas, st)
+                            : launch_weights<FMT_INT4, DT_F16>(wp, head_size, rows, tiles, ctas, st);
+  return dtype == DT_BF16 ? launch_weights<FMT_K8V4, DT_BF16>(wp, head_size, rows, tiles, ctas, st)
+                          : launch_weights<FMT_K8V4, DT_F16>(wp, head_size, rows, tiles, ctas, st);
 }
