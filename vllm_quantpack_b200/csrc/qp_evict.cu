@@ -12,20 +12,6 @@
 
 namespace qp {
 
-// Division of an index below 2^31 by a launch constant d: i / d = i m >> (31 + s) with s = ceil(log2 d) and
-// m = floor(2^(31 + s) / d) + 1, which fits 32 bits and is off by less than 2^s / 2^(31 + s) a unit of i.
-struct FastDiv {
-  uint32_t m;
-  int s, d;
-  explicit FastDiv(int divisor) : m(0), s(0), d(divisor) {
-    while ((1ll << s) < divisor) ++s;
-    m = static_cast<uint32_t>((1ull << (31 + s)) / static_cast<uint64_t>(divisor) + 1);
-  }
-  __device__ __forceinline__ int div(int i) const {
-    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(i)) * m) >> (31 + s));
-  }
-};
-
 struct EvictParams {
   uint8_t* cache;
   FastDiv block_size;

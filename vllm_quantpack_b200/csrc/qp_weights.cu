@@ -14,11 +14,16 @@
 //   warp 0        query tiles: one bulk copy of a prepared record (both terms in the operand's swizzled layout, the
 //                 rows' -lse and mask bounds) into a ring; a tile that the next keys use again is not copied again;
 //   warp 1        issues HS / 8 MMAs of K 16 per 128 keys and query tile, S^T double-buffered;
-//   warps 2-5     keys: cp.async of the key half of the cells only, 8 bytes a lane (the values in between are not
-//                 read: a cell's key part is not 16-byte aligned), then thread = key: codes to exact fp16 in TMEM;
-//   warps 6-13    thread = key and half of the columns: exponentials, the sum, one add to global memory per key.
+//   4 or 8 warps  key operand: thread = key, its codes to exact fp16 in TMEM (two sets on alternate tiles where few rows
+//                 make the conversion the longest role);
+//   8 warps       thread = key: exponentials, the sum over the rows, one add to global memory per key; two sets, one
+//                 for each S^T buffer;
+//   1 or 4 warps  cp.async of the key part of the cells, 8 bytes a lane (a cell's key part is not 16-byte aligned),
+//                 into a ring of raw stages. With the 64-byte fetch hint the values in between mostly stay in HBM:
+//                 75 % of the cells' bytes are read at int4 and head 256, 62 % at head 512, 94 % at head 128 (without
+//                 the hint, in 128-byte fetches, all of them).
 // Few rows (up to 32, decoding): a tile of 128 keys meets one query tile, two key tiles alternate in TMEM; bound by
-// the bytes of the key half (136 of 264 at int4, head 256). Many rows (prompts): a group of two key tiles stays in
+// the bytes of the key part. Many rows (prompts): a group of two key tiles stays in
 // TMEM while all query tiles that see it stream through L2, so a query tile's bytes serve 256 keys; bound by the MMAs
 // (two terms) at head 256, by the exponentials (16 a cycle and SM) at head 128.
 // The (key group, query tile) steps of all sequences and KV heads are cut evenly over the CTAs; where a cut falls
@@ -41,6 +46,7 @@ struct WeightParams {
   const float* lse;  // [tokens][nq]
   float* weights;
   int64_t w_block, w_slot, w_head;  // element strides
+  FastDiv block_size;
   int max_q, max_k;  // bounds of the lengths that the launch was sized for
   // workspace: prepared query tiles; per CTA the sums of a group's parts and what they are
   uint8_t* qrec;
@@ -49,7 +55,6 @@ struct WeightParams {
 };
 
 constexpr int WT_KEYS = 128;     // keys of a tile (TMEM lanes)
-constexpr int WT_THREADS = 448;  // 14 warps
 constexpr int WT_SMALL_ROWS = 32;  // query rows of a KV head up to which a sequence is one query tile
 
 // NR: rows of a query tile; KT: key tiles of a group; MANY: a sequence may have several query tiles
@@ -70,19 +75,28 @@ struct WT {
   static constexpr int HEAD = ROWS + 12 * NR;      // then {score scale, least last key, greatest first key}
   static constexpr int QREC = (HEAD + 16 + 1023) / 1024 * 1024;
   static constexpr int QS = HS == 512 && (!MANY || FMT == FMT_K8V4) ? 1 : 2;
+  // warps: 0 query tiles, 1 MMA, then the key operand, the weights and the raw keys (many rows keep a key tile long
+  // enough for one converting set and one loading warp)
+  static constexpr int CSETS = MANY || SLOTS == 1 ? 1 : 2;
+  static constexpr int LOADERS = MANY ? 1 : 4;
+  static constexpr int W_SUM = 2 + 4 * CSETS, W_LOAD = W_SUM + 8;
+  static constexpr int THREADS = 32 * (W_LOAD + LOADERS);
+  static constexpr int RUN_STEPS = (16 * PIECES + 31) / 32;  // cp.asyncs of a lane for 16 keys
   static constexpr int MISC = 4 * 128 * 4 + 2 * 128 * 4 + 32 * 8 + 64;
   static constexpr int RS0 = (231000 - QS * QREC - MISC) / STAGE;
-  static constexpr int RS = RS0 > 4 ? 4 : RS0;
+  // even, so that a stage's phases are all seen by one converting set
+  static constexpr int RS = RS0 >= 6 ? 6 : RS0 >= 4 ? 4 : 2;
   static constexpr int OFF_RAW = QS * QREC;
   static constexpr int OFF_KP = OFF_RAW + RS * STAGE;  // [4][128] float: key scale of the last tiles
   static constexpr int OFF_RED = OFF_KP + 4 * 128 * 4;  // [2][128] float: the second half's sums
   static constexpr int OFF_BAR = OFF_RED + 2 * 128 * 4;
   static constexpr int OFF_TMEM = OFF_BAR + 32 * 8;
   static constexpr int BYTES = OFF_TMEM + 64;  // the TMEM address, then where the share starts
-  static_assert(RS >= 2 && BYTES <= 232448, "shared memory");
+  static_assert(RS0 >= 2 && BYTES <= 232448, "shared memory");
 };
 
-enum { T_Q_FULL = 0, T_Q_EMPTY = 2, T_K_FULL = 4, T_K_FREE = 6, T_S_FULL = 8, T_S_FREE = 10, T_FINAL = 12 };
+enum { T_Q_FULL = 0, T_Q_EMPTY = 2, T_K_FULL = 4, T_K_FREE = 6, T_S_FULL = 8, T_S_FREE = 10, T_FINAL = 12,
+       T_RAW_FULL = 13, T_RAW_EMPTY = 19 };  // [RS <= 6] each
 
 // ---- the steps of a sequence: for each key group, the query tiles [first, end) with a row that sees one of its keys
 struct Steps {
@@ -104,6 +118,11 @@ __device__ __forceinline__ Steps steps_of(const WeightParams& wp, int seq) {
 template <int NR, int GK>
 __device__ __forceinline__ void tiles_seeing(const Steps& s, int g, int& first, int& end) {
   const int lo = g * GK, hi = min(lo + GK, s.n) - 1;  // the group's keys
+  if (s.window == 0 && lo <= s.vis_base) {
+    first = 0;
+    end = s.ntq;
+    return;
+  }
   const int tok = max(0, lo - s.vis_base);
   first = tok >= s.qlen ? s.ntq : static_cast<int>(static_cast<int64_t>(tok) * s.group / NR);
   end = s.ntq;
@@ -178,7 +197,7 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 }
 
 // The sequence that unit `at` lies in, units(b) units a sequence, and what comes before it of units and tiles(b).
-// scratch: 2 x 16 words of 64 bits. All `threads` threads call it and get the same answer in found[0..2].
+// scratch: 2 x 24 words of 64 bits. All `threads` threads call it and get the same answer in found[0..2].
 template <class U, class T>
 __device__ __forceinline__ void find_sequence(int num_seqs, int threads, int64_t at, U&& units, T&& tiles,
                                               int64_t* scratch, int64_t* found) {
@@ -199,17 +218,17 @@ __device__ __forceinline__ void find_sequence(int num_seqs, int threads, int64_t
     __syncthreads();
     if (lane == 31) {
       scratch[warp] = iu;
-      scratch[16 + warp] = it;
+      scratch[24 + warp] = it;
     }
     __syncthreads();
     int64_t bu = before_u, bt = before_t;
     for (int w = 0; w < warps; ++w) {
       if (w < warp) {
         bu += scratch[w];
-        bt += scratch[16 + w];
+        bt += scratch[24 + w];
       }
       before_u += scratch[w];
-      before_t += scratch[16 + w];
+      before_t += scratch[24 + w];
     }
     const int64_t start = bu + iu - u;
     if (start <= at && at < start + u) {
@@ -222,21 +241,21 @@ __device__ __forceinline__ void find_sequence(int num_seqs, int threads, int64_t
   __syncthreads();
 }
 
-template <int NR, int GK>
+template <int NR, int GK, int THREADS>
 __device__ __forceinline__ void find_start(const WeightParams& wp, int64_t* scratch, ShareStart* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const auto units = [&](int b) { return count_steps<NR, GK>(steps_of<NR>(wp, b)) * wp.d.nkv; };
   int64_t total = 0;
-  for (int b = tid; b < wp.d.num_seqs; b += WT_THREADS) total += units(b);
+  for (int b = tid; b < wp.d.num_seqs; b += THREADS) total += units(b);
   total = warp_sum64(total);
   if (lane == 0) scratch[warp] = total;
   __syncthreads();
   total = 0;
-  for (int w = 0; w < WT_THREADS / 32; ++w) total += scratch[w];
+  for (int w = 0; w < THREADS / 32; ++w) total += scratch[w];
   const int64_t share = (total + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * share, hi = min(lo + share, total);
-  int64_t* found = scratch + 32;
+  int64_t* found = scratch + 48;
   if (lo < hi)
-    find_sequence(wp.d.num_seqs, WT_THREADS, lo, units, [&](int b) { return steps_of<NR>(wp, b).ntq; }, scratch,
+    find_sequence(wp.d.num_seqs, THREADS, lo, units, [&](int b) { return steps_of<NR>(wp, b).ntq; }, scratch,
                   found);
   if (tid == 0) {
     out->lo = lo;
@@ -281,7 +300,7 @@ __global__ void __launch_bounds__(256) weights_qprep_kernel(const WeightParams w
   using EL = Elem<DT>;
   constexpr int E = HS / 32, RW = NR / 8;  // channels a lane, rows a warp
   const DecodeParams& p = wp.d;
-  __shared__ int64_t scratch[36];
+  __shared__ int64_t scratch[52];
   __shared__ float wmax[8];
   __shared__ int wvis[8], wlo[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y;
@@ -291,12 +310,12 @@ __global__ void __launch_bounds__(256) weights_qprep_kernel(const WeightParams w
       seq = 0;
       qt = blockIdx.x;
     } else {
-      if (tid == 0) scratch[32] = -1;
+      if (tid == 0) scratch[48] = -1;
       const auto tiles = [&](int b) { return static_cast<int64_t>(steps_of<NR>(wp, b).ntq); };
-      find_sequence(p.num_seqs, 256, blockIdx.x, tiles, tiles, scratch, scratch + 32);
-      if (scratch[32] < 0) return;
-      seq = static_cast<int>(scratch[32]);
-      qt = static_cast<int>(blockIdx.x - scratch[33]);
+      find_sequence(p.num_seqs, 256, blockIdx.x, tiles, tiles, scratch, scratch + 48);
+      if (scratch[48] < 0) return;
+      seq = static_cast<int>(scratch[48]);
+      qt = static_cast<int>(blockIdx.x - scratch[49]);
     }
   }
   const Steps s = steps_of<NR>(wp, seq);
@@ -409,13 +428,8 @@ __global__ void __launch_bounds__(256) weights_qprep_kernel(const WeightParams w
   }
 }
 
-__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global.L2::64B [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // 32 TMEM columns (64 channels) of a key's exact codes from 32 (int4) or 64 (k8v4) bytes
@@ -451,18 +465,17 @@ __device__ __forceinline__ void key_columns(const uint8_t* codes, uint32_t lo_bi
 }
 
 // The call's own tokens have no earlier weight; a page of the others may be shared by sequences of the call.
-__device__ __forceinline__ void add_weight(const WeightParams& wp, int seq, int kvh, int key, int vis_base, float w) {
-  const DecodeParams& p = wp.d;
-  const int b = key / p.block_size;
-  float* at = wp.weights + p.block_table[seq * p.bt_stride + b] * wp.w_block +
-              static_cast<int64_t>(key - b * p.block_size) * wp.w_slot + kvh * wp.w_head;
+__device__ __forceinline__ void add_weight(const WeightParams& wp, int32_t page, int block, int kvh, int key,
+                                           int vis_base, float w) {
+  float* at = wp.weights + page * wp.w_block + static_cast<int64_t>(key - block * wp.block_size.d) * wp.w_slot +
+              kvh * wp.w_head;
   if (key >= vis_base) *at = w;
   else atomicAdd(at, w);
 }
 
 // ---------------------------------------------------------------------------------------------------- K4
 template <int FMT, int HS, int NR, int KT, bool MANY, bool CAP>
-__global__ void __launch_bounds__(WT_THREADS, 1) weights_kernel(const WeightParams wp) {
+__global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weights_kernel(const WeightParams wp) {
   using W = WT<FMT, HS, NR, KT, MANY>;
   using CL = typename W::CL;
   constexpr int GK = WT_KEYS * KT, SLOTS = W::SLOTS, RS = W::RS, QS = W::QS;
@@ -481,7 +494,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_kernel(const WeightPara
       mbar_init(&bars[T_K_FULL + i], 4);
       mbar_init(&bars[T_K_FREE + i], 1);
       mbar_init(&bars[T_S_FULL + i], 1);
-      mbar_init(&bars[T_S_FREE + i], 8);
+      mbar_init(&bars[T_S_FREE + i], 4);
+    }
+    for (int i = 0; i < RS; ++i) {
+      mbar_init(&bars[T_RAW_FULL + i], 32 * W::LOADERS);
+      mbar_init(&bars[T_RAW_EMPTY + i], 4);
     }
     mbar_init(&bars[T_FINAL], 1);
     fence_mbar_init();
@@ -490,7 +507,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_kernel(const WeightPara
     tmem_alloc(tmem_slot, W::COLS);
     tmem_relinquish();
   }
-  find_start<NR, GK>(wp, reinterpret_cast<int64_t*>(smem + W::OFF_RAW), &start);
+  find_start<NR, GK, W::THREADS>(wp, reinterpret_cast<int64_t*>(smem + W::OFF_RAW), &start);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -580,57 +597,22 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_kernel(const WeightPara
     if (elect_one()) umma_commit(&bars[T_FINAL]);
     __syncwarp();
     mbar_wait_spin(&bars[T_FINAL], 0);  // every MMA has completed before TMEM goes
-  } else if (warp < 6) {
-    // ------------------------------------------------------------------ keys (thread = key = TMEM lane)
-    const int ct = tid - 64, quarter = warp & 3, kl = 32 * quarter + lane;
+  } else if (warp < W::W_SUM) {
+    // ------------------------------------------------------------------ key operand (thread = key = TMEM lane)
+    const int quarter = warp & 3, set = (warp - 2) >> 2, kl = 32 * quarter + lane;
     float* kp = reinterpret_cast<float*>(smem + W::OFF_KP);
-    // the raw stages are filled one walk ahead of the conversion
-    Walk<NR, GK> ahead = walk;
-    int at = 0, kt_ahead = 0;
-    const uint8_t* run = nullptr;  // lanes 0-7: the tile's 16-cell runs
-    const auto issue = [&](int tile) {
-      if (at == kt_ahead) {
-        at = 0;
-        kt_ahead = ahead.next(wp) ? min(KT, (ahead.s.n - ahead.g * GK + WT_KEYS - 1) / WT_KEYS) : 0;
-      }
-      if (at < kt_ahead) {
-        const int k0 = ahead.g * GK + at * WT_KEYS, mine = k0 + 16 * (lane & 7);
-        run = nullptr;
-        if (mine < ahead.s.n) {
-          const int32_t page = p.block_table[ahead.seq * p.bt_stride + mine / p.block_size];
-          run = p.cache + static_cast<int64_t>(page) * p.block_stride +
-                static_cast<int64_t>(ahead.kvh) * p.head_stride +
-                static_cast<int64_t>(mine % p.block_size) * CL::BYTES;
-        }
-        uint8_t* dst = smem + W::OFF_RAW + (tile % RS) * W::STAGE;
-#pragma unroll 4
-        for (int e = 0; e < W::PIECES; ++e) {
-          const int idx = e * 128 + ct, key = idx / W::PIECES, piece = idx - key * W::PIECES;
-          const uint8_t* src = reinterpret_cast<const uint8_t*>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(run), key >> 4));
-          if (k0 + key < ahead.s.n) cp_async8(dst + idx * 8, src + (key & 15) * CL::BYTES + piece * 8);
-        }
-        ++at;
-      }
-      cp_async_commit();
-    };
     int tile = 0;
-    bool leave = false;  // set for all four warps at once
-#pragma unroll
-    for (int i = 0; i < RS - 1; ++i) issue(i);
-    while (!leave && walk.next(wp)) {
+    while (ok && walk.next(wp)) {
       const int kt = tiles_in();
       for (int t = 0; t < kt; ++t, ++tile) {
-        cp_async_wait<RS - 2>();
-        leave = named_bar_or(1, 128, !ok);
-        if (leave) break;
-        issue(tile + RS - 1);  // into the stage that every thread has left
-        const int sl = tile % SLOTS;
-        if (tile >= SLOTS)
-          ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_K_FREE + sl], (tile / SLOTS - 1) & 1));
-        if (!ok) continue;
+        if (W::CSETS == 2 && (tile & 1) != set) continue;
+        const int sl = tile % SLOTS, st = tile % RS;
+        ok = mbar_wait_spin(&bars[T_RAW_FULL + st], (tile / RS) & 1);
+        if (ok && tile >= SLOTS) ok = mbar_wait_spin(&bars[T_K_FREE + sl], (tile / SLOTS - 1) & 1);
+        ok = !__any_sync(0xffffffffu, !ok);
+        if (!ok) break;
         tc_fence_after();
-        const uint8_t* raw = smem + W::OFF_RAW + (tile % RS) * W::STAGE + kl * W::KEY;
+        const uint8_t* raw = smem + W::OFF_RAW + st * W::STAGE + kl * W::KEY;
         const uint32_t word = *reinterpret_cast<const uint32_t*>(raw + CL::KB);
         const uint32_t zp = FMT == FMT_INT4 ? word & 0xFu : 0u;
         const uint32_t lo1 = 0x6400u | zp, hi1 = 0xD400u | (zp << 4);  // 1024 + zp, -(64 + zp)
@@ -641,32 +623,40 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_kernel(const WeightPara
           key_columns<FMT>(raw + c * (CL::KB / (HS / 64)), lo1 | (lo1 << 16), hi1 | (hi1 << 16), a);
           tmem_st32u(ta + 32 * c, a);
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         const bool valid = walk.g * GK + t * WT_KEYS + kl < walk.s.n;
         kp[(tile & 3) * 128 + kl] = !valid ? 0.f : __uint_as_float(FMT == FMT_INT4 ? word & 0xFFFFFFF0u : word);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[T_K_FULL + sl]);
+        if (lane == 0) {
+          mbar_arrive(&bars[T_RAW_EMPTY + st]);
+          mbar_arrive(&bars[T_K_FULL + sl]);
+        }
       }
     }
-    cp_async_wait<0>();
-  } else {
-    // ------------------------------------------------------------------ weights (thread = key, half of the columns)
-    constexpr int NH = NR / 2, CH = NH < 16 ? NH : 16;  // columns a thread, and at a time
-    const int quarter = warp & 3, half = (warp - 6) >> 2, kl = 32 * quarter + lane;
-    const uint32_t ta = tmem + W::S + half * NH + (static_cast<uint32_t>(32 * quarter) << 16);
+  } else if (warp < W::W_LOAD) {
+    // ------------------------------------------------------------------ weights (thread = key)
+    // Set b takes the jobs of S^T buffer b: one tile of each pair of a group, or every other job of a lone tile.
+    constexpr int CH = NR < 16 ? NR : 16;  // columns at a time
+    const int quarter = warp & 3, set = (warp - W::W_SUM) >> 2, kl = 32 * quarter + lane;
+    const uint32_t ta = tmem + W::S + set * NR + (static_cast<uint32_t>(32 * quarter) << 16);
     const float* kp = reinterpret_cast<const float*>(smem + W::OFF_KP);
     float* red = reinterpret_cast<float*>(smem + W::OFF_RED);
     const float capl = CAP ? p.softcap * LOG2E : 0.f, cap_k = CAP ? 2.f * LOG2E / capl : 0.f;
     int64_t cur = -1;
-    int loads = 0, jobs = 0, tiles = 0, sums = 0;
+    int loads = 0, jobs = 0, tiles = 0;
     int4 rec_head = make_int4(0, 0, 0, 0), rec_tail = make_int4(0, 0, 0, 0);
-    while (walk.next(wp)) {
-      const int kt = tiles_in();
-      float ks[KT];
-      float2 sum[KT];
-#pragma unroll
-      for (int t = 0; t < KT; ++t) sum[t] = make_float2(0.f, 0.f);
+    while ((ok || MANY) && walk.next(wp)) {  // (a set that gave up still meets the barrier below)
+      const int kt = tiles_in(), mine = kt == 2 ? (set - jobs) & 1 : 0;  // this set's tile of the group
+      const int k0 = walk.g * GK + mine * WT_KEYS, key = k0 + kl;
+      // a lone tile is this set's to write if it has its first job
+      const bool writes = kt == 2 || (jobs & 1) == set;
+      const int block = wp.block_size.div(key);
+      int32_t page = 0;  // on its way while the scores are made
+      if (writes && key < walk.s.n) page = p.block_table[static_cast<int64_t>(walk.seq) * p.bt_stride + block];
+      float ks = 0.f;
+      bool first = true;
+      float2 sum = make_float2(0.f, 0.f);
       for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
         const int64_t id = tile_id(qt);
         if (id != cur) {
@@ -674,87 +664,133 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_kernel(const WeightPara
           cur = id;
           ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_Q_FULL + loads % QS], (loads / QS) & 1));
           ++loads;
+          if (!ok) break;
         }
+        const int j = jobs + (kt == 2 ? (set - jobs) & 1 : 0);  // this set's job of the query tile, if it has one
+        jobs += kt;
+        if ((j & 1) != set) continue;
+        ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_S_FULL + set], (j / 2) & 1));
+        if (!ok) break;
+        tc_fence_after();
         const uint8_t* rec = smem + ((loads - 1) % QS) * W::QREC;
         const float4 hd = *reinterpret_cast<const float4*>(rec + W::HEAD);
-        const float* nl = reinterpret_cast<const float*>(rec + W::ROWS) + half * NH;
-        const int* vis = reinterpret_cast<const int*>(rec + W::ROWS) + NR + half * NH;
+        const float* nl = reinterpret_cast<const float*>(rec + W::ROWS);
+        const int* vis = reinterpret_cast<const int*>(rec + W::ROWS) + NR;
+        if (first) ks = kp[((tiles + mine) & 3) * 128 + kl];
+        first = false;
+        const float k1 = ks * hd.x;
+        const bool masked = k0 + WT_KEYS - 1 > __float_as_int(hd.y) || k0 < __float_as_int(hd.z);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          if (t >= kt || !ok) break;
-          const int b = jobs & 1, k0 = walk.g * GK + t * WT_KEYS;
-          ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_S_FULL + b], (jobs / 2) & 1));
-          ++jobs;
-          if (!ok) break;
-          tc_fence_after();
-          if (qt == walk.qa) ks[t] = kp[((tiles + t) & 3) * 128 + kl];
-          const float k1 = ks[t] * hd.x;
-          const bool masked = k0 + WT_KEYS - 1 > __float_as_int(hd.y) || k0 < __float_as_int(hd.z);
+        for (int c0 = 0; c0 < NR; c0 += CH) {
+          float sc[CH];
+          tmem_ld_cols<CH>(ta + c0, sc);
+          if (c0 + CH == NR) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[T_S_FREE + set]);
+          }
 #pragma unroll
-          for (int c0 = 0; c0 < NH; c0 += CH) {
-            float sc[CH];
-            tmem_ld_cols<CH>(ta + b * NR + c0, sc);
-            if (c0 + CH == NH) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars[T_S_FREE + b]);
+          for (int c = 0; c < CH; c += 4) {
+            const float4 l4 = *reinterpret_cast<const float4*>(nl + c0 + c);
+            float2 x[2];
+            if constexpr (!CAP) {
+              x[0] = __ffma2_rn(make_float2(sc[c], sc[c + 1]), make_float2(k1, k1), make_float2(l4.x, l4.y));
+              x[1] = __ffma2_rn(make_float2(sc[c + 2], sc[c + 3]), make_float2(k1, k1), make_float2(l4.z, l4.w));
+            } else {
+              x[0] = make_float2(softcap_log2(sc[c] * k1, capl, cap_k) + l4.x,
+                                 softcap_log2(sc[c + 1] * k1, capl, cap_k) + l4.y);
+              x[1] = make_float2(softcap_log2(sc[c + 2] * k1, capl, cap_k) + l4.z,
+                                 softcap_log2(sc[c + 3] * k1, capl, cap_k) + l4.w);
             }
-#pragma unroll
-            for (int c = 0; c < CH; c += 4) {
-              const float4 l4 = *reinterpret_cast<const float4*>(nl + c0 + c);
-              float2 x[2];
-              if constexpr (!CAP) {
-                x[0] = __ffma2_rn(make_float2(sc[c], sc[c + 1]), make_float2(k1, k1), make_float2(l4.x, l4.y));
-                x[1] = __ffma2_rn(make_float2(sc[c + 2], sc[c + 3]), make_float2(k1, k1), make_float2(l4.z, l4.w));
-              } else {
-                x[0] = make_float2(softcap_log2(sc[c] * k1, capl, cap_k) + l4.x,
-                                   softcap_log2(sc[c + 1] * k1, capl, cap_k) + l4.y);
-                x[1] = make_float2(softcap_log2(sc[c + 2] * k1, capl, cap_k) + l4.z,
-                                   softcap_log2(sc[c + 3] * k1, capl, cap_k) + l4.w);
-              }
-              if (masked) {
-                const int key = k0 + kl;
-                const int4 v = *reinterpret_cast<const int4*>(vis + c0 + c);
-                const int4 f = *reinterpret_cast<const int4*>(vis + NR + c0 + c);
-                if (key > v.x || key < f.x) x[0].x = -INFINITY;
-                if (key > v.y || key < f.y) x[0].y = -INFINITY;
-                if (key > v.z || key < f.z) x[1].x = -INFINITY;
-                if (key > v.w || key < f.w) x[1].y = -INFINITY;
-              }
-              sum[t] = __fadd2_rn(sum[t], make_float2(fast_exp2(x[0].x), fast_exp2(x[0].y)));
-              sum[t] = __fadd2_rn(sum[t], make_float2(fast_exp2(x[1].x), fast_exp2(x[1].y)));
+            if (masked) {
+              const int4 v = *reinterpret_cast<const int4*>(vis + c0 + c);
+              const int4 f = *reinterpret_cast<const int4*>(vis + NR + c0 + c);
+              if (key > v.x || key < f.x) x[0].x = -INFINITY;
+              if (key > v.y || key < f.y) x[0].y = -INFINITY;
+              if (key > v.z || key < f.z) x[1].x = -INFINITY;
+              if (key > v.w || key < f.w) x[1].y = -INFINITY;
             }
+            sum = __fadd2_rn(sum, make_float2(fast_exp2(x[0].x), fast_exp2(x[0].y)));
+            sum = __fadd2_rn(sum, make_float2(fast_exp2(x[1].x), fast_exp2(x[1].y)));
           }
         }
       }
-      // the halves' sums meet; whole groups go to the weights, parts of one to the workspace
+      tiles += kt;
+      // whole groups go to the weights, parts of one to the workspace
       const bool head = walk.qa > walk.first, tail = walk.qb < walk.end;
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        if (t >= kt) break;
-        float* r = red + (sums++ & 1) * 128;
-        if (half == 1) r[kl] = sum[t].x + sum[t].y;
-        if (named_bar_or(2, 256, !ok)) {
-          ok = false;
-          break;
-        }
-        const int key = walk.g * GK + t * WT_KEYS + kl;
-        if (half == 0 && key < walk.s.n) {
-          const float w = sum[t].x + sum[t].y + r[kl];
-          if (head || tail)
-            wp.part[(static_cast<int64_t>(blockIdx.x) * 2 + (head ? 0 : 1)) * 256 + t * WT_KEYS + kl] = w;
-          else add_weight(wp, walk.seq, walk.kvh, key, walk.s.vis_base, w);
-        }
+      float w = sum.x + sum.y;
+      if (MANY && kt == 1) {  // both sets had jobs of the tile
+        if (!writes) red[kl] = w;
+        if (named_bar_or(1, 256, !ok)) break;
+        if (writes) w += red[kl];
+        named_bar_or(1, 256, false);  // read before the next lone tile's
       }
-      if (!ok) break;
+      if (ok && writes && key < walk.s.n) {
+        if (head || tail)
+          wp.part[(static_cast<int64_t>(blockIdx.x) * 2 + (head ? 0 : 1)) * 256 + mine * WT_KEYS + kl] = w;
+        else add_weight(wp, page, block, walk.kvh, key, walk.s.vis_base, w);
+      }
       if (head) rec_head = make_int4(1, tail, 0, 0);
       else if (tail) rec_tail = make_int4(1, walk.seq, walk.kvh, walk.g);
-      tiles += kt;
     }
-    if (MANY && warp == 6 && lane == 0) {
+    if (MANY && warp == W::W_SUM && lane == 0) {
       wp.records[2 * blockIdx.x] = rec_head;
       wp.records[2 * blockIdx.x + 1] = rec_tail;
     }
+  } else {
+    // ------------------------------------------------------------------ raw keys
+    // A warp copies 8 / LOADERS of a tile's 16-cell runs: lane l the 8-byte pieces l, l + 32, ... of a run's key parts.
+    constexpr int RUNS = 8 / W::LOADERS;
+    const int r0 = (warp - W::W_LOAD) * RUNS;
+    uint32_t at[W::RUN_STEPS];  // of each piece: key << 16 | byte from the run's first cell
+#pragma unroll
+    for (int e = 0; e < W::RUN_STEPS; ++e) {
+      const int idx = e * 32 + lane, key = idx / W::PIECES;
+      at[e] = static_cast<uint32_t>(key << 16 | (key * CL::BYTES + (idx - key * W::PIECES) * 8));
+    }
+    // lane r < 8 looks up run r of the next tile while the present one is issued
+    int t = 0, kt = 0, keys = 0;  // keys: of the tile that next_src belongs to, 0 at the end
+    const uint8_t* next_src = nullptr;
+    const auto look = [&]() {
+      if (t == kt) {
+        t = 0;
+        kt = walk.next(wp) ? tiles_in() : 0;
+      }
+      keys = 0;
+      if (t < kt) {
+        const int k0 = walk.g * GK + t * WT_KEYS, mine = k0 + 16 * (lane & 7);
+        keys = min(WT_KEYS, walk.s.n - k0);
+        if (mine < walk.s.n) {
+          const int b = wp.block_size.div(mine);
+          next_src = p.cache + p.block_table[walk.seq * p.bt_stride + b] * p.block_stride +
+                     static_cast<int64_t>(walk.kvh) * p.head_stride +
+                     static_cast<int64_t>(mine - b * p.block_size) * CL::BYTES;
+        }
+        ++t;
+      }
+    };
+    look();
+    for (int tile = 0; keys > 0; ++tile) {
+      const int st = tile % RS, have = keys;
+      const uint8_t* const src = next_src;
+      look();
+      if (tile >= RS) ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_RAW_EMPTY + st], (tile / RS - 1) & 1));
+      if (!ok) break;
+      const uint32_t dst = smem_u32(smem + W::OFF_RAW + st * W::STAGE) + lane * 8;
+#pragma unroll 1
+      for (int r = r0; r < r0 + RUNS; ++r) {
+        const uint8_t* base = reinterpret_cast<const uint8_t*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
+        const int keys_r = have - 16 * r;  // a run past the sequence is not there
+#pragma unroll
+        for (int e = 0; e < W::RUN_STEPS; ++e)
+          if (static_cast<int>(at[e] >> 16) < min(keys_r, 16))
+            cp_async8(dst + r * 16 * W::KEY + e * 256, base + (at[e] & 0xFFFFu));
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[T_RAW_FULL + st]))
+                   : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -778,7 +814,10 @@ __global__ void __launch_bounds__(GK) weights_fold_kernel(const WeightParams wp)
   }
   const Steps s = steps_of<16>(wp, rec.y);
   const int key = rec.w * GK + threadIdx.x;
-  if (key < s.n) add_weight(wp, rec.y, rec.z, key, s.vis_base, w);
+  if (key >= s.n) return;
+  const int block = wp.block_size.div(key);
+  add_weight(wp, wp.d.block_table[static_cast<int64_t>(rec.y) * wp.d.bt_stride + block], block, rec.z, key, s.vis_base,
+             w);
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -811,7 +850,7 @@ static int launch_weights_t(const WeightParams& wp, int64_t tiles, int ctas, cud
   int rc = check_launch("attention weights q prep");
   if (rc) return rc;
   cudaLaunchAttribute pdl[1];
-  cudaLaunchConfig_t cfg = wt_config(dim3(ctas), WT_THREADS, W::BYTES, st, pdl);
+  cudaLaunchConfig_t cfg = wt_config(dim3(ctas), W::THREADS, W::BYTES, st, pdl);
   cudaError_t e = cudaLaunchKernelEx(&cfg, weights_kernel<FMT, HS, NR, KT, MANY, CAP>, wp);
   if (e == cudaSuccess && MANY) {
     cfg = wt_config(dim3(ctas), WT_KEYS * KT, 0, st, pdl);
@@ -915,7 +954,7 @@ extern "C" int qp_accumulate_attn_weights(int fmt, int dtype, const void* q, int
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)
     return set_error(QP_ERR_WORKSPACE, "attention weights: workspace of %lld bytes < %lld", (long long)workspace_bytes,
                      (long long)need);
-  WeightParams wp{};
+  WeightParams wp{{}, nullptr, nullptr, 0, 0, 0, FastDiv(block_size)};
   DecodeParams& dp = wp.d;
   dp.q = q;
   dp.q_st = q_stride_token;
