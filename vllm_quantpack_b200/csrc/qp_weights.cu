@@ -13,7 +13,8 @@
 // One persistent CTA per SM; roles:
 //   warp 0        query tiles: one bulk copy of a prepared record (both terms in the operand's swizzled layout, the
 //                 rows' -lse and mask bounds) into a ring; a tile that the next keys use again is not copied again;
-//   warp 1        issues HS / 8 MMAs of K 16 per 128 keys and query tile, S^T double-buffered;
+//   2 warps       (the second and the last, on different SM sub-partitions) issue HS / 8 MMAs of K 16 per 128 keys and
+//                 query tile, each into its own S^T buffer, so that one's waits pass while the other's MMAs run;
 //   4 or 8 warps  key operand: thread = key, its codes to exact fp16 in TMEM (two sets on alternate tiles where few rows
 //                 make the conversion the longest role);
 //   8 warps       thread = key: exponentials, the sum over the rows, one add to global memory per key; two sets, one
@@ -75,17 +76,20 @@ struct WT {
   static constexpr int HEAD = ROWS + 12 * NR;      // then {score scale, least last key, greatest first key}
   static constexpr int QREC = (HEAD + 16 + 1023) / 1024 * 1024;
   static constexpr int QS = HS == 512 && (!MANY || FMT == FMT_K8V4) ? 1 : 2;
-  // warps: 0 query tiles, 1 MMA, then the key operand, the weights and the raw keys (many rows keep a key tile long
-  // enough for one converting set and one loading warp)
+  // warps: 0 query tiles, 1 MMA, then the key operand, the weights, the raw keys (many rows keep a key tile long enough
+  // for one converting set and one loading warp) and the second MMA warp
   static constexpr int CSETS = MANY || SLOTS == 1 ? 1 : 2;
-  static constexpr int LOADERS = MANY ? 1 : 4;
+  // where a TMEM slot is not always the same MMA warp's, both follow every tile (so that neither misses a phase)
+  static constexpr bool BOTH = MANY || SLOTS == 1;
   static constexpr int W_SUM = 2 + 4 * CSETS, W_LOAD = W_SUM + 8;
-  static constexpr int THREADS = 32 * (W_LOAD + LOADERS);
   static constexpr int RUN_STEPS = (16 * PIECES + 31) / 32;  // cp.asyncs of a lane for 16 keys
   static constexpr int MISC = 4 * 128 * 4 + 2 * 128 * 4 + 32 * 8 + 64;
   static constexpr int RS0 = (231000 - QS * QREC - MISC) / STAGE;
-  // even, so that a stage's phases are all seen by one converting set
-  static constexpr int RS = RS0 >= 6 ? 6 : RS0 >= 4 ? 4 : 2;
+  // raw stages, and loading warps (tiles in turn): a stage is always filled by the same warp and emptied by the same
+  // converting set, which so see all of its phases
+  static constexpr int RS = RS0 >= 8 ? 8 : RS0 >= 4 ? 4 : 2;
+  static constexpr int LOADERS = MANY ? 1 : RS < 4 ? 2 : 4;
+  static constexpr int W_MMA1 = W_LOAD + LOADERS, THREADS = 32 * (W_MMA1 + 1);
   static constexpr int OFF_RAW = QS * QREC;
   static constexpr int OFF_KP = OFF_RAW + RS * STAGE;  // [4][128] float: key scale of the last tiles
   static constexpr int OFF_RED = OFF_KP + 4 * 128 * 4;  // [2][128] float: the second half's sums
@@ -96,13 +100,13 @@ struct WT {
 };
 
 enum { T_Q_FULL = 0, T_Q_EMPTY = 2, T_K_FULL = 4, T_K_FREE = 6, T_S_FULL = 8, T_S_FREE = 10, T_FINAL = 12,
-       T_RAW_FULL = 13, T_RAW_EMPTY = 19 };  // [RS <= 6] each
+       T_RAW_FULL = 13, T_RAW_EMPTY = 21 };  // [RS <= 8] each
 
 // ---- the steps of a sequence: for each key group, the query tiles [first, end) with a row that sees one of its keys
 struct Steps {
-  int qlen, n, vis_base, group, window, ntq;
+  int qlen, n, vis_base, group, window, ntq, groups;
 };
-template <int NR>
+template <int NR, int GK>
 __device__ __forceinline__ Steps steps_of(const WeightParams& wp, int seq) {
   const DecodeParams& p = wp.d;
   Steps s;
@@ -113,6 +117,7 @@ __device__ __forceinline__ Steps steps_of(const WeightParams& wp, int seq) {
   s.window = p.window;
   s.ntq = (min(s.qlen, wp.max_q) * p.group + NR - 1) / NR;
   if (s.qlen <= 0 || s.n < 0) s.n = s.ntq = 0;
+  s.groups = (s.n + GK - 1) / GK;
   return s;
 }
 template <int NR, int GK>
@@ -131,16 +136,14 @@ __device__ __forceinline__ void tiles_seeing(const Steps& s, int g, int& first, 
     end = last < 0 ? first : max(first, static_cast<int>((static_cast<int64_t>(last + 1) * s.group - 1) / NR) + 1);
   }
 }
-template <int GK>
-__device__ __forceinline__ int groups_of(const Steps& s) { return (s.n + GK - 1) / GK; }
 // group from which the steps of a group are not all ntq any more (no window)
 template <int GK>
 __device__ __forceinline__ int full_groups(const Steps& s) {
-  return s.window > 0 ? 0 : max(0, min(groups_of<GK>(s), s.vis_base < 0 ? 0 : s.vis_base / GK + 1));
+  return s.window > 0 ? 0 : max(0, min(s.groups, s.vis_base < 0 ? 0 : s.vis_base / GK + 1));
 }
 template <int NR, int GK>
 __device__ __forceinline__ int64_t count_steps(const Steps& s) {
-  const int full = full_groups<GK>(s), groups = groups_of<GK>(s);
+  const int full = full_groups<GK>(s), groups = s.groups;
   int64_t t = static_cast<int64_t>(full) * s.ntq;
   for (int g = full; g < groups; ++g) {
     int a, b;
@@ -155,7 +158,7 @@ template <int NR, int GK>
 struct Walk {
   int seq, kvh, g, qa, qb, first, end;  // the segment; all query tiles of its group
   int qbase;                            // query tiles of the sequences before
-  int64_t left;                         // steps of the share not yet handed out
+  int left;                             // steps of the share not yet handed out
   Steps s;
 
   __device__ __forceinline__ bool next(const WeightParams& wp) {
@@ -163,17 +166,17 @@ struct Walk {
     for (;;) {
       if (qb < end) {  // the group's tiles from qb on
         qa = qb;
-        qb = static_cast<int>(min(static_cast<int64_t>(end), qa + left));
+        qb = min(end, qa + left);
         left -= qb - qa;
         return true;
       }
-      if (++g >= groups_of<GK>(s)) {
+      if (++g >= s.groups) {
         g = 0;
         if (++kvh == wp.d.nkv) {
           kvh = 0;
           do {
             qbase += s.ntq;
-            s = steps_of<NR>(wp, ++seq);
+            s = steps_of<NR, GK>(wp, ++seq);
           } while (s.n == 0);
         }
       }
@@ -244,7 +247,7 @@ __device__ __forceinline__ void find_sequence(int num_seqs, int threads, int64_t
 template <int NR, int GK, int THREADS>
 __device__ __forceinline__ void find_start(const WeightParams& wp, int64_t* scratch, ShareStart* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const auto units = [&](int b) { return count_steps<NR, GK>(steps_of<NR>(wp, b)) * wp.d.nkv; };
+  const auto units = [&](int b) { return count_steps<NR, GK>(steps_of<NR, GK>(wp, b)) * wp.d.nkv; };
   int64_t total = 0;
   for (int b = tid; b < wp.d.num_seqs; b += THREADS) total += units(b);
   total = warp_sum64(total);
@@ -255,7 +258,7 @@ __device__ __forceinline__ void find_start(const WeightParams& wp, int64_t* scra
   const int64_t share = (total + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * share, hi = min(lo + share, total);
   int64_t* found = scratch + 48;
   if (lo < hi)
-    find_sequence(wp.d.num_seqs, THREADS, lo, units, [&](int b) { return steps_of<NR>(wp, b).ntq; }, scratch,
+    find_sequence(wp.d.num_seqs, THREADS, lo, units, [&](int b) { return steps_of<NR, GK>(wp, b).ntq; }, scratch,
                   found);
   if (tid == 0) {
     out->lo = lo;
@@ -263,7 +266,7 @@ __device__ __forceinline__ void find_start(const WeightParams& wp, int64_t* scra
     if (lo < hi) {
       out->seq = static_cast<int>(found[0]);
       out->qbase = static_cast<int>(found[2]);
-      const Steps s = steps_of<NR>(wp, out->seq);
+      const Steps s = steps_of<NR, GK>(wp, out->seq);
       const int64_t each = count_steps<NR, GK>(s);
       out->kvh = static_cast<int>((lo - found[1]) / each);
       int64_t u = (lo - found[1]) % each;
@@ -311,14 +314,14 @@ __global__ void __launch_bounds__(256) weights_qprep_kernel(const WeightParams w
       qt = blockIdx.x;
     } else {
       if (tid == 0) scratch[48] = -1;
-      const auto tiles = [&](int b) { return static_cast<int64_t>(steps_of<NR>(wp, b).ntq); };
+      const auto tiles = [&](int b) { return static_cast<int64_t>(steps_of<NR, WT_KEYS>(wp, b).ntq); };
       find_sequence(p.num_seqs, 256, blockIdx.x, tiles, tiles, scratch, scratch + 48);
       if (scratch[48] < 0) return;
       seq = static_cast<int>(scratch[48]);
       qt = static_cast<int>(blockIdx.x - scratch[49]);
     }
   }
-  const Steps s = steps_of<NR>(wp, seq);
+  const Steps s = steps_of<NR, WT_KEYS>(wp, seq);
   if (qt >= s.ntq) return;
   // the record's place: the sequences' tiles in a row (one place each where none has more), KV heads inside
   uint8_t* rec = wp.qrec + (static_cast<int64_t>(blockIdx.x) * p.nkv + kvh) * W::QREC;
@@ -490,17 +493,17 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[T_Q_FULL + i], 1);
-      mbar_init(&bars[T_Q_EMPTY + i], 1 + 8);
+      mbar_init(&bars[T_Q_EMPTY + i], 2 + 8);
       mbar_init(&bars[T_K_FULL + i], 4);
-      mbar_init(&bars[T_K_FREE + i], 1);
+      mbar_init(&bars[T_K_FREE + i], W::BOTH ? 2 : 1);
       mbar_init(&bars[T_S_FULL + i], 1);
       mbar_init(&bars[T_S_FREE + i], 4);
     }
     for (int i = 0; i < RS; ++i) {
-      mbar_init(&bars[T_RAW_FULL + i], 32 * W::LOADERS);
+      mbar_init(&bars[T_RAW_FULL + i], 32);
       mbar_init(&bars[T_RAW_EMPTY + i], 4);
     }
-    mbar_init(&bars[T_FINAL], 1);
+    mbar_init(&bars[T_FINAL], 2);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -513,13 +516,13 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Walk<NR, GK> walk;
-  walk.left = start.hi - start.lo;
+  walk.left = static_cast<int>(start.hi - start.lo);
   if (walk.left > 0) {
     walk.seq = start.seq;
     walk.kvh = start.kvh;
     walk.g = start.g;
     walk.qbase = start.qbase;
-    walk.s = steps_of<NR>(wp, start.seq);
+    walk.s = steps_of<NR, GK>(wp, start.seq);
     tiles_seeing<NR, GK>(walk.s, walk.g, walk.first, walk.end);
     walk.qb = start.q;
   }
@@ -551,9 +554,10 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     }
     // the copies in flight land before the CTA's shared memory can go away
     for (int k = max(0, loads - QS); k < loads; ++k) mbar_wait_bounded(&bars[T_Q_FULL + k % QS], (k / QS) & 1);
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMAs
+  } else if (warp == 1 || warp == W::W_MMA1) {
+    // ------------------------------------------------------------------ MMAs (this warp's: the jobs of its S^T buffer)
     constexpr uint32_t ID = f16_idesc(128, NR, false);
+    const int buf = warp == 1 ? 0 : 1;
     int64_t cur = -1;
     int loads = 0, jobs = 0, tiles = 0;  // query tiles seen, S buffers filled, key tiles before this group
     const auto wait = [&](int bar, uint32_t parity) {
@@ -572,24 +576,30 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
         }
         const uint64_t qd = sw128_desc(smem_u32(smem + ((loads - 1) % QS) * W::QREC), 16, 1024);
         for (int t = 0; t < kt && ok; ++t, ++jobs) {
-          const int tile = tiles + t, sl = tile % SLOTS, b = jobs & 1;
-          if (qt == walk.qa) wait(T_K_FULL + sl, (tile / SLOTS) & 1);
-          if (jobs >= 2) wait(T_S_FREE + b, (jobs / 2 - 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t ak = tmem + sl * W::ACOLS, sd = tmem + W::S + b * NR;
+          const int tile = tiles + t, sl = tile % SLOTS;
+          const bool own = (jobs & 1) == buf;
+          if (qt == walk.qa && (own || W::BOTH)) wait(T_K_FULL + sl, (tile / SLOTS) & 1);
+          if (own) {
+            if (jobs >= 2) wait(T_S_FREE + buf, (jobs / 2 - 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t ak = tmem + sl * W::ACOLS, sd = tmem + W::S + buf * NR;
 #pragma unroll
-            for (int term = 0; term < 2; ++term)
+              for (int term = 0; term < 2; ++term)
 #pragma unroll
-              for (int c = 0; c < HS / 16; ++c)
-                umma_f16_ts(sd, ak + 8 * c,
-                            qd + static_cast<uint64_t>((term * W::TERM + (c >> 2) * W::ATOM + (c & 3) * 32) >> 4), ID,
-                            (term | c) ? 1u : 0u);
-            umma_commit(&bars[T_S_FULL + b]);
-            if (qt == walk.qb - 1) umma_commit(&bars[T_K_FREE + sl]);
+                for (int c = 0; c < HS / 16; ++c)
+                  umma_f16_ts(sd, ak + 8 * c,
+                              qd + static_cast<uint64_t>((term * W::TERM + (c >> 2) * W::ATOM + (c & 3) * 32) >> 4),
+                              ID, (term | c) ? 1u : 0u);
+              umma_commit(&bars[T_S_FULL + buf]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (ok && qt == walk.qb - 1 && (own || W::BOTH)) {  // this warp's MMAs on the tile are all issued
+            if (elect_one()) umma_commit(&bars[T_K_FREE + sl]);
+            __syncwarp();
+          }
         }
       }
       tiles += kt;
@@ -739,52 +749,55 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     }
   } else {
     // ------------------------------------------------------------------ raw keys
-    // A warp copies 8 / LOADERS of a tile's 16-cell runs: lane l the 8-byte pieces l, l + 32, ... of a run's key parts.
-    constexpr int RUNS = 8 / W::LOADERS;
-    const int r0 = (warp - W::W_LOAD) * RUNS;
+    // A warp copies every LOADERS-th tile: lane l the 8-byte pieces l, l + 32, ... of each 16-cell run's key parts.
+    const int me = warp - W::W_LOAD;
     uint32_t at[W::RUN_STEPS];  // of each piece: key << 16 | byte from the run's first cell
 #pragma unroll
     for (int e = 0; e < W::RUN_STEPS; ++e) {
       const int idx = e * 32 + lane, key = idx / W::PIECES;
       at[e] = static_cast<uint32_t>(key << 16 | (key * CL::BYTES + (idx - key * W::PIECES) * 8));
     }
-    // lane r < 8 looks up run r of the next tile while the present one is issued
-    int t = 0, kt = 0, keys = 0;  // keys: of the tile that next_src belongs to, 0 at the end
-    const uint8_t* next_src = nullptr;
-    const auto look = [&]() {
-      if (t == kt) {
-        t = 0;
-        kt = walk.next(wp) ? tiles_in() : 0;
-      }
-      keys = 0;
-      if (t < kt) {
-        const int k0 = walk.g * GK + t * WT_KEYS, mine = k0 + 16 * (lane & 7);
-        keys = min(WT_KEYS, walk.s.n - k0);
-        if (mine < walk.s.n) {
-          const int b = wp.block_size.div(mine);
-          next_src = p.cache + p.block_table[walk.seq * p.bt_stride + b] * p.block_stride +
-                     static_cast<int64_t>(walk.kvh) * p.head_stride +
-                     static_cast<int64_t>(mine - b * p.block_size) * CL::BYTES;
+    // lane r < 8 reads the page of run r of the warp's next tile while the present one is copied
+    int t = 0, kt = 0, next = -1;  // next: the tile last looked at
+    int k_next = 0, kvh_next = 0, keys_next = 0;
+    int32_t page_next = 0;
+    const auto look = [&]() {  // on to the warp's next tile; keys_next 0 at the end
+      keys_next = 0;
+      do {
+        if (t == kt) {
+          t = 0;
+          kt = walk.next(wp) ? tiles_in() : 0;
+          if (kt == 0) return;
         }
         ++t;
-      }
+        ++next;
+      } while (next % W::LOADERS != me);
+      const int k0 = walk.g * GK + (t - 1) * WT_KEYS;
+      k_next = k0 + 16 * (lane & 7);
+      kvh_next = walk.kvh;
+      keys_next = min(WT_KEYS, walk.s.n - k0);
+      if (k_next < walk.s.n)
+        page_next = p.block_table[static_cast<int64_t>(walk.seq) * p.bt_stride + wp.block_size.div(k_next)];
     };
     look();
-    for (int tile = 0; keys > 0; ++tile) {
-      const int st = tile % RS, have = keys;
-      const uint8_t* const src = next_src;
+    while (keys_next > 0) {
+      const int tile = next, st = tile % RS, have = keys_next;
+      const uint8_t* const src =
+          p.cache + page_next * p.block_stride + kvh_next * p.head_stride +
+          static_cast<int64_t>(k_next - wp.block_size.div(k_next) * wp.block_size.d) * CL::BYTES;
       look();
       if (tile >= RS) ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_RAW_EMPTY + st], (tile / RS - 1) & 1));
       if (!ok) break;
       const uint32_t dst = smem_u32(smem + W::OFF_RAW + st * W::STAGE) + lane * 8;
 #pragma unroll 1
-      for (int r = r0; r < r0 + RUNS; ++r) {
+      for (int r = 0; r < 8; ++r) {
         const uint8_t* base = reinterpret_cast<const uint8_t*>(
             __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
-        const int keys_r = have - 16 * r;  // a run past the sequence is not there
+        const int keys_r = min(have - 16 * r, 16);  // a run past the sequence is not there
+        if (keys_r <= 0) break;
 #pragma unroll
         for (int e = 0; e < W::RUN_STEPS; ++e)
-          if (static_cast<int>(at[e] >> 16) < min(keys_r, 16))
+          if (static_cast<int>(at[e] >> 16) < keys_r)
             cp_async8(dst + r * 16 * W::KEY + e * 256, base + (at[e] & 0xFFFFu));
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[T_RAW_FULL + st]))
@@ -812,7 +825,7 @@ __global__ void __launch_bounds__(GK) weights_fold_kernel(const WeightParams wp)
     w += wp.part[static_cast<int64_t>(c) * 512 + threadIdx.x];
     if (!r.y) break;
   }
-  const Steps s = steps_of<16>(wp, rec.y);
+  const Steps s = steps_of<16, GK>(wp, rec.y);
   const int key = rec.w * GK + threadIdx.x;
   if (key >= s.n) return;
   const int block = wp.block_size.div(key);
