@@ -153,25 +153,47 @@ __device__ __forceinline__ int64_t count_steps(const Steps& s) {
   return t;
 }
 
-// Walks a CTA's share: segments (sequence, KV head, group, query tiles [qa, qb)) in order. Every role runs its own.
-template <int NR, int GK>
+// Few rows: a sequence's one query tile sees the groups [first_group, s.groups) (all of them without a window).
+template <int GK>
+__device__ __forceinline__ int first_group(const Steps& s) {
+  if (s.ntq == 0) return s.groups;
+  if (s.window == 0) return 0;
+  const int lo = max(0, s.vis_base - s.window + 1);
+  return lo >= s.n ? s.groups : lo / GK;
+}
+template <int NR, int GK, bool MANY>
+__device__ __forceinline__ int64_t steps_in(const Steps& s) {
+  if constexpr (MANY) return count_steps<NR, GK>(s);
+  else return s.groups - first_group<GK>(s);
+}
+
+// Walks a CTA's share in order; every role runs its own. Many rows: a segment is a group and the query tiles [qa, qb) of
+// its [first, end). Few rows: the groups [g, g1) of a (sequence, KV head).
+template <int NR, int GK, bool MANY>
 struct Walk {
-  int seq, kvh, g, qa, qb, first, end;  // the segment; all query tiles of its group
-  int qbase;                            // query tiles of the sequences before
-  int left;                             // steps of the share not yet handed out
+  int seq, kvh, g, g1, qa, qb, first, end;
+  int qbase;  // query tiles of the sequences before
+  int left;   // steps of the share not yet handed out
   Steps s;
 
   __device__ __forceinline__ bool next(const WeightParams& wp) {
     if (left <= 0) return false;
     for (;;) {
-      if (qb < end) {  // the group's tiles from qb on
-        qa = qb;
-        qb = min(end, qa + left);
-        left -= qb - qa;
+      if constexpr (MANY) {
+        if (qb < end) {  // the group's tiles from qb on
+          qa = qb;
+          qb = min(end, qa + left);
+          left -= qb - qa;
+          return true;
+        }
+        ++g;
+      } else if (g1 < s.groups) {
+        g = g1;
+        g1 = min(s.groups, g + left);
+        left -= g1 - g;
         return true;
       }
-      if (++g >= s.groups) {
-        g = 0;
+      if (!MANY || g >= s.groups) {
         if (++kvh == wp.d.nkv) {
           kvh = 0;
           do {
@@ -179,9 +201,13 @@ struct Walk {
             s = steps_of<NR, GK>(wp, ++seq);
           } while (s.n == 0);
         }
+        g = MANY ? 0 : first_group<GK>(s);
       }
-      tiles_seeing<NR, GK>(s, g, first, end);
-      qb = first;
+      g1 = MANY ? g + 1 : g;
+      if constexpr (MANY) {
+        tiles_seeing<NR, GK>(s, g, first, end);
+        qb = first;
+      }
     }
   }
 };
@@ -244,10 +270,10 @@ __device__ __forceinline__ void find_sequence(int num_seqs, int threads, int64_t
   __syncthreads();
 }
 
-template <int NR, int GK, int THREADS>
+template <int NR, int GK, bool MANY, int THREADS>
 __device__ __forceinline__ void find_start(const WeightParams& wp, int64_t* scratch, ShareStart* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const auto units = [&](int b) { return count_steps<NR, GK>(steps_of<NR, GK>(wp, b)) * wp.d.nkv; };
+  const auto units = [&](int b) { return steps_in<NR, GK, MANY>(steps_of<NR, GK>(wp, b)) * wp.d.nkv; };
   int64_t total = 0;
   for (int b = tid; b < wp.d.num_seqs; b += THREADS) total += units(b);
   total = warp_sum64(total);
@@ -267,15 +293,16 @@ __device__ __forceinline__ void find_start(const WeightParams& wp, int64_t* scra
       out->seq = static_cast<int>(found[0]);
       out->qbase = static_cast<int>(found[2]);
       const Steps s = steps_of<NR, GK>(wp, out->seq);
-      const int64_t each = count_steps<NR, GK>(s);
+      const int64_t each = steps_in<NR, GK, MANY>(s);
       out->kvh = static_cast<int>((lo - found[1]) / each);
       int64_t u = (lo - found[1]) % each;
       const int full = full_groups<GK>(s);
-      int g, a, b;
-      if (u < static_cast<int64_t>(full) * s.ntq) {
+      int g, a = 0, b;
+      if (!MANY) {
+        g = first_group<GK>(s) + static_cast<int>(u);
+      } else if (u < static_cast<int64_t>(full) * s.ntq) {
         g = static_cast<int>(u / s.ntq);
         u -= static_cast<int64_t>(g) * s.ntq;
-        a = 0;
       } else {
         u -= static_cast<int64_t>(full) * s.ntq;
         for (g = full;; ++g) {
@@ -510,27 +537,35 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     tmem_alloc(tmem_slot, W::COLS);
     tmem_relinquish();
   }
-  find_start<NR, GK, W::THREADS>(wp, reinterpret_cast<int64_t*>(smem + W::OFF_RAW), &start);
+  find_start<NR, GK, MANY, W::THREADS>(wp, reinterpret_cast<int64_t*>(smem + W::OFF_RAW), &start);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walk<NR, GK> walk;
+  Walk<NR, GK, MANY> walk;
   walk.left = static_cast<int>(start.hi - start.lo);
   if (walk.left > 0) {
     walk.seq = start.seq;
     walk.kvh = start.kvh;
     walk.g = start.g;
+    walk.g1 = MANY ? start.g + 1 : start.g;
     walk.qbase = start.qbase;
     walk.s = steps_of<NR, GK>(wp, start.seq);
-    tiles_seeing<NR, GK>(walk.s, walk.g, walk.first, walk.end);
-    walk.qb = start.q;
+    if constexpr (MANY) {
+      tiles_seeing<NR, GK>(walk.s, walk.g, walk.first, walk.end);
+      walk.qb = start.q;
+    }
   }
-  const auto tiles_in = [&]() {  // key tiles of the group that hold keys
-    return min(KT, (walk.s.n - walk.g * GK + WT_KEYS - 1) / WT_KEYS);
+  const auto tiles_in = [&](int g) {  // key tiles of group g that hold keys
+    return KT == 1 ? 1 : min(KT, (walk.s.n - g * GK + WT_KEYS - 1) / WT_KEYS);
   };
   const auto tile_id = [&](int qt) { return static_cast<int64_t>(MANY ? walk.qbase + qt : walk.seq) * p.nkv + walk.kvh; };
   bool ok = true;
+  const auto wait = [&](int bar, uint32_t parity) {
+    if (ok) ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[bar], parity));
+  };
+  // Jobs (one key tile, one query tile) and key tiles are counted alike in every role: job j uses S^T buffer j & 1, key
+  // tile i raw stage i % RS and TMEM slot i % SLOTS. With few rows a tile is one job, of the same number.
 
   if (warp == 0) {
     // ------------------------------------------------------------------ query tiles
@@ -538,18 +573,18 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     int64_t cur = -1;
     int loads = 0;
     while (ok && walk.next(wp)) {
-      for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
+      for (int qt = MANY ? walk.qa : 0; qt < (MANY ? walk.qb : 1) && ok; ++qt) {
         const int64_t id = tile_id(qt);
         if (id == cur) continue;
         cur = id;
         const int st = loads % QS;
-        if (loads >= QS) ok = !__any_sync(0xffffffffu, !mbar_wait_bounded(&bars[T_Q_EMPTY + st], (loads / QS - 1) & 1));
+        if (loads >= QS) wait(T_Q_EMPTY + st, (loads / QS - 1) & 1);
         if (ok && lane == 0) {
           mbar_arrive_expect_tx(&bars[T_Q_FULL + st], W::QREC);
           bulk_g2s(smem + st * W::QREC, wp.qrec + id * W::QREC, W::QREC, &bars[T_Q_FULL + st]);
         }
         __syncwarp();
-        ++loads;
+        loads += ok;
       }
     }
     // the copies in flight land before the CTA's shared memory can go away
@@ -559,50 +594,62 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     constexpr uint32_t ID = f16_idesc(128, NR, false);
     const int buf = warp == 1 ? 0 : 1;
     int64_t cur = -1;
-    int loads = 0, jobs = 0, tiles = 0;  // query tiles seen, S buffers filled, key tiles before this group
-    const auto wait = [&](int bar, uint32_t parity) {
-      if (ok) ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[bar], parity));
+    int loads = 0, jobs = 0, tiles = 0;
+    uint64_t qd = 0;
+    const auto enter = [&](int64_t id) {  // the jobs from here on are of query tile id
+      if (id == cur) return;
+      cur = id;
+      if (loads > 0 && elect_one()) umma_commit(&bars[T_Q_EMPTY + (loads - 1) % QS]);
+      __syncwarp();
+      wait(T_Q_FULL + loads % QS, (loads / QS) & 1);
+      qd = sw128_desc(smem_u32(smem + (loads % QS) * W::QREC), 16, 1024);
+      ++loads;
+    };
+    const auto job = [&](int j, int sl) {
+      if (j >= 2) wait(T_S_FREE + buf, (j / 2 - 1) & 1);
+      if (!ok) return;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t ak = tmem + sl * W::ACOLS, sd = tmem + W::S + buf * NR;
+#pragma unroll
+        for (int term = 0; term < 2; ++term)
+#pragma unroll
+          for (int c = 0; c < HS / 16; ++c)
+            umma_f16_ts(sd, ak + 8 * c,
+                        qd + static_cast<uint64_t>((term * W::TERM + (c >> 2) * W::ATOM + (c & 3) * 32) >> 4), ID,
+                        (term | c) ? 1u : 0u);
+        umma_commit(&bars[T_S_FULL + buf]);
+      }
+      __syncwarp();
+    };
+    const auto release = [&](int sl) {  // this warp's MMAs on the tile are all issued
+      if (ok && elect_one()) umma_commit(&bars[T_K_FREE + sl]);
+      __syncwarp();
     };
     while (ok && walk.next(wp)) {
-      const int kt = tiles_in();
-      for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
-        const int64_t id = tile_id(qt);
-        if (id != cur) {
-          if (loads > 0 && elect_one()) umma_commit(&bars[T_Q_EMPTY + (loads - 1) % QS]);
-          __syncwarp();
-          cur = id;
-          wait(T_Q_FULL + loads % QS, (loads / QS) & 1);
-          ++loads;
+      if constexpr (!MANY) {
+        enter(tile_id(0));
+        for (int n = walk.g1 - walk.g; n > 0 && ok; --n, ++tiles) {
+          const bool own = (tiles & 1) == buf;
+          if (!own && !W::BOTH) continue;
+          const int sl = tiles % SLOTS;
+          wait(T_K_FULL + sl, (tiles / SLOTS) & 1);
+          if (own) job(tiles, sl);
+          release(sl);
         }
-        const uint64_t qd = sw128_desc(smem_u32(smem + ((loads - 1) % QS) * W::QREC), 16, 1024);
-        for (int t = 0; t < kt && ok; ++t, ++jobs) {
-          const int tile = tiles + t, sl = tile % SLOTS;
-          const bool own = (jobs & 1) == buf;
-          if (qt == walk.qa && (own || W::BOTH)) wait(T_K_FULL + sl, (tile / SLOTS) & 1);
-          if (own) {
-            if (jobs >= 2) wait(T_S_FREE + buf, (jobs / 2 - 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t ak = tmem + sl * W::ACOLS, sd = tmem + W::S + buf * NR;
-#pragma unroll
-              for (int term = 0; term < 2; ++term)
-#pragma unroll
-                for (int c = 0; c < HS / 16; ++c)
-                  umma_f16_ts(sd, ak + 8 * c,
-                              qd + static_cast<uint64_t>((term * W::TERM + (c >> 2) * W::ATOM + (c & 3) * 32) >> 4),
-                              ID, (term | c) ? 1u : 0u);
-              umma_commit(&bars[T_S_FULL + buf]);
-            }
-            __syncwarp();
-          }
-          if (ok && qt == walk.qb - 1 && (own || W::BOTH)) {  // this warp's MMAs on the tile are all issued
-            if (elect_one()) umma_commit(&bars[T_K_FREE + sl]);
-            __syncwarp();
+      } else {
+        const int kt = tiles_in(walk.g);
+        for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
+          enter(tile_id(qt));
+          for (int t = 0; t < kt && ok; ++t, ++jobs) {
+            const int sl = (tiles + t) % SLOTS;
+            if (qt == walk.qa) wait(T_K_FULL + sl, ((tiles + t) / SLOTS) & 1);
+            if ((jobs & 1) == buf) job(jobs, sl);
+            if (qt == walk.qb - 1) release(sl);
           }
         }
+        tiles += kt;
       }
-      tiles += kt;
     }
     if (elect_one()) umma_commit(&bars[T_FINAL]);
     __syncwarp();
@@ -613,40 +660,42 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     float* kp = reinterpret_cast<float*>(smem + W::OFF_KP);
     int tile = 0;
     while (ok && walk.next(wp)) {
-      const int kt = tiles_in();
-      for (int t = 0; t < kt; ++t, ++tile) {
-        if (W::CSETS == 2 && (tile & 1) != set) continue;
-        const int sl = tile % SLOTS, st = tile % RS;
-        ok = mbar_wait_spin(&bars[T_RAW_FULL + st], (tile / RS) & 1);
-        if (ok && tile >= SLOTS) ok = mbar_wait_spin(&bars[T_K_FREE + sl], (tile / SLOTS - 1) & 1);
-        ok = !__any_sync(0xffffffffu, !ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint8_t* raw = smem + W::OFF_RAW + st * W::STAGE + kl * W::KEY;
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(raw + CL::KB);
-        const uint32_t zp = FMT == FMT_INT4 ? word & 0xFu : 0u;
-        const uint32_t lo1 = 0x6400u | zp, hi1 = 0xD400u | (zp << 4);  // 1024 + zp, -(64 + zp)
-        const uint32_t ta = tmem + sl * W::ACOLS + (static_cast<uint32_t>(32 * quarter) << 16);
+      for (int g = walk.g; g < walk.g1 && ok; ++g) {
+        const int kt = tiles_in(g);
+        for (int t = 0; t < kt && ok; ++t, ++tile) {
+          if (W::CSETS == 2 && (tile & 1) != set) continue;
+          const int sl = tile % SLOTS, st = tile % RS;
+          wait(T_RAW_FULL + st, (tile / RS) & 1);
+          if (tile >= SLOTS) wait(T_K_FREE + sl, (tile / SLOTS - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint8_t* raw = smem + W::OFF_RAW + st * W::STAGE + kl * W::KEY;
+          const uint32_t word = *reinterpret_cast<const uint32_t*>(raw + CL::KB);
+          const uint32_t zp = FMT == FMT_INT4 ? word & 0xFu : 0u;
+          const uint32_t lo1 = 0x6400u | zp, hi1 = 0xD400u | (zp << 4);  // 1024 + zp, -(64 + zp)
+          const uint32_t ta = tmem + sl * W::ACOLS + (static_cast<uint32_t>(32 * quarter) << 16);
 #pragma unroll 1
-        for (int c = 0; c < HS / 64; ++c) {
-          uint32_t a[32];
-          key_columns<FMT>(raw + c * (CL::KB / (HS / 64)), lo1 | (lo1 << 16), hi1 | (hi1 << 16), a);
-          tmem_st32u(ta + 32 * c, a);
-        }
-        const bool valid = walk.g * GK + t * WT_KEYS + kl < walk.s.n;
-        kp[(tile & 3) * 128 + kl] = !valid ? 0.f : __uint_as_float(FMT == FMT_INT4 ? word & 0xFFFFFFF0u : word);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars[T_RAW_EMPTY + st]);
-          mbar_arrive(&bars[T_K_FULL + sl]);
+          for (int c = 0; c < HS / 64; ++c) {
+            uint32_t a[32];
+            key_columns<FMT>(raw + c * (CL::KB / (HS / 64)), lo1 | (lo1 << 16), hi1 | (hi1 << 16), a);
+            tmem_st32u(ta + 32 * c, a);
+          }
+          const bool valid = g * GK + t * WT_KEYS + kl < walk.s.n;
+          kp[(tile & 3) * 128 + kl] = !valid ? 0.f : __uint_as_float(FMT == FMT_INT4 ? word & 0xFFFFFFF0u : word);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bars[T_RAW_EMPTY + st]);
+            mbar_arrive(&bars[T_K_FULL + sl]);
+          }
         }
       }
     }
   } else if (warp < W::W_LOAD) {
     // ------------------------------------------------------------------ weights (thread = key)
-    // Set b takes the jobs of S^T buffer b: one tile of each pair of a group, or every other job of a lone tile.
+    // Set b takes the jobs of S^T buffer b: every other tile (few rows), one tile of each pair of a group, or every other
+    // job of a lone tile.
     constexpr int CH = NR < 16 ? NR : 16;  // columns at a time
     const int quarter = warp & 3, set = (warp - W::W_SUM) >> 2, kl = 32 * quarter + lane;
     const uint32_t ta = tmem + W::S + set * NR + (static_cast<uint32_t>(32 * quarter) << 16);
@@ -656,92 +705,110 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     int64_t cur = -1;
     int loads = 0, jobs = 0, tiles = 0;
     int4 rec_head = make_int4(0, 0, 0, 0), rec_tail = make_int4(0, 0, 0, 0);
-    while ((ok || MANY) && walk.next(wp)) {  // (a set that gave up still meets the barrier below)
-      const int kt = tiles_in(), mine = kt == 2 ? (set - jobs) & 1 : 0;  // this set's tile of the group
-      const int k0 = walk.g * GK + mine * WT_KEYS, key = k0 + kl;
-      // a lone tile is this set's to write if it has its first job
-      const bool writes = kt == 2 || (jobs & 1) == set;
-      const int block = wp.block_size.div(key);
-      int32_t page = 0;  // on its way while the scores are made
-      if (writes && key < walk.s.n) page = p.block_table[static_cast<int64_t>(walk.seq) * p.bt_stride + block];
-      float ks = 0.f;
-      bool first = true;
-      float2 sum = make_float2(0.f, 0.f);
-      for (int qt = walk.qa; qt < walk.qb && ok; ++qt) {
-        const int64_t id = tile_id(qt);
-        if (id != cur) {
-          if (loads > 0 && lane == 0) mbar_arrive(&bars[T_Q_EMPTY + (loads - 1) % QS]);
-          cur = id;
-          ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_Q_FULL + loads % QS], (loads / QS) & 1));
-          ++loads;
-          if (!ok) break;
-        }
-        const int j = jobs + (kt == 2 ? (set - jobs) & 1 : 0);  // this set's job of the query tile, if it has one
-        jobs += kt;
-        if ((j & 1) != set) continue;
-        ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_S_FULL + set], (j / 2) & 1));
-        if (!ok) break;
-        tc_fence_after();
-        const uint8_t* rec = smem + ((loads - 1) % QS) * W::QREC;
-        const float4 hd = *reinterpret_cast<const float4*>(rec + W::HEAD);
-        const float* nl = reinterpret_cast<const float*>(rec + W::ROWS);
-        const int* vis = reinterpret_cast<const int*>(rec + W::ROWS) + NR;
-        if (first) ks = kp[((tiles + mine) & 3) * 128 + kl];
-        first = false;
-        const float k1 = ks * hd.x;
-        const bool masked = k0 + WT_KEYS - 1 > __float_as_int(hd.y) || k0 < __float_as_int(hd.z);
+    const uint8_t* rec = smem;
+    const auto enter = [&](int64_t id) {
+      if (id == cur) return;
+      cur = id;
+      if (loads > 0 && lane == 0) mbar_arrive(&bars[T_Q_EMPTY + (loads - 1) % QS]);
+      wait(T_Q_FULL + loads % QS, (loads / QS) & 1);
+      rec = smem + (loads % QS) * W::QREC;
+      ++loads;
+    };
+    // job j's scores: the sum over the rows of the key's weights, k0 the tile's first key, ks the key's scale
+    const auto job = [&](int j, int tile, int k0, float2& sum) {
+      wait(T_S_FULL + set, (j / 2) & 1);
+      if (!ok) return;
+      tc_fence_after();
+      const float ks = kp[(tile & 3) * 128 + kl];
+      const float4 hd = *reinterpret_cast<const float4*>(rec + W::HEAD);
+      const float* nl = reinterpret_cast<const float*>(rec + W::ROWS);
+      const int* vis = reinterpret_cast<const int*>(rec + W::ROWS) + NR;
+      const float k1 = ks * hd.x;
+      const bool masked = k0 + WT_KEYS - 1 > __float_as_int(hd.y) || k0 < __float_as_int(hd.z);
 #pragma unroll
-        for (int c0 = 0; c0 < NR; c0 += CH) {
-          float sc[CH];
-          tmem_ld_cols<CH>(ta + c0, sc);
-          if (c0 + CH == NR) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[T_S_FREE + set]);
+      for (int c0 = 0; c0 < NR; c0 += CH) {
+        float sc[CH];
+        tmem_ld_cols<CH>(ta + c0, sc);
+        if (c0 + CH == NR) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[T_S_FREE + set]);
+        }
+        float2 x[CH / 2];
+#pragma unroll
+        for (int c = 0; c < CH; c += 4) {
+          const float4 l4 = *reinterpret_cast<const float4*>(nl + c0 + c);
+          if constexpr (!CAP) {
+            x[c / 2] = __ffma2_rn(make_float2(sc[c], sc[c + 1]), make_float2(k1, k1), make_float2(l4.x, l4.y));
+            x[c / 2 + 1] = __ffma2_rn(make_float2(sc[c + 2], sc[c + 3]), make_float2(k1, k1), make_float2(l4.z, l4.w));
+          } else {
+            x[c / 2] = make_float2(softcap_log2(sc[c] * k1, capl, cap_k) + l4.x,
+                                   softcap_log2(sc[c + 1] * k1, capl, cap_k) + l4.y);
+            x[c / 2 + 1] = make_float2(softcap_log2(sc[c + 2] * k1, capl, cap_k) + l4.z,
+                                       softcap_log2(sc[c + 3] * k1, capl, cap_k) + l4.w);
           }
+        }
+        if (masked) {
+          const int key = k0 + kl;
 #pragma unroll
           for (int c = 0; c < CH; c += 4) {
-            const float4 l4 = *reinterpret_cast<const float4*>(nl + c0 + c);
-            float2 x[2];
-            if constexpr (!CAP) {
-              x[0] = __ffma2_rn(make_float2(sc[c], sc[c + 1]), make_float2(k1, k1), make_float2(l4.x, l4.y));
-              x[1] = __ffma2_rn(make_float2(sc[c + 2], sc[c + 3]), make_float2(k1, k1), make_float2(l4.z, l4.w));
-            } else {
-              x[0] = make_float2(softcap_log2(sc[c] * k1, capl, cap_k) + l4.x,
-                                 softcap_log2(sc[c + 1] * k1, capl, cap_k) + l4.y);
-              x[1] = make_float2(softcap_log2(sc[c + 2] * k1, capl, cap_k) + l4.z,
-                                 softcap_log2(sc[c + 3] * k1, capl, cap_k) + l4.w);
-            }
-            if (masked) {
-              const int4 v = *reinterpret_cast<const int4*>(vis + c0 + c);
-              const int4 f = *reinterpret_cast<const int4*>(vis + NR + c0 + c);
-              if (key > v.x || key < f.x) x[0].x = -INFINITY;
-              if (key > v.y || key < f.y) x[0].y = -INFINITY;
-              if (key > v.z || key < f.z) x[1].x = -INFINITY;
-              if (key > v.w || key < f.w) x[1].y = -INFINITY;
-            }
-            sum = __fadd2_rn(sum, make_float2(fast_exp2(x[0].x), fast_exp2(x[0].y)));
-            sum = __fadd2_rn(sum, make_float2(fast_exp2(x[1].x), fast_exp2(x[1].y)));
+            const int4 v = *reinterpret_cast<const int4*>(vis + c0 + c);
+            const int4 f = *reinterpret_cast<const int4*>(vis + NR + c0 + c);
+            if (key > v.x || key < f.x) x[c / 2].x = -INFINITY;
+            if (key > v.y || key < f.y) x[c / 2].y = -INFINITY;
+            if (key > v.z || key < f.z) x[c / 2 + 1].x = -INFINITY;
+            if (key > v.w || key < f.w) x[c / 2 + 1].y = -INFINITY;
           }
         }
+#pragma unroll
+        for (int c = 0; c < CH / 2; ++c) sum = __fadd2_rn(sum, make_float2(fast_exp2(x[c].x), fast_exp2(x[c].y)));
       }
-      tiles += kt;
-      // whole groups go to the weights, parts of one to the workspace
-      const bool head = walk.qa > walk.first, tail = walk.qb < walk.end;
-      float w = sum.x + sum.y;
-      if (MANY && kt == 1) {  // both sets had jobs of the tile
-        if (!writes) red[kl] = w;
-        if (named_bar_or(1, 256, !ok)) break;
-        if (writes) w += red[kl];
-        named_bar_or(1, 256, false);  // read before the next lone tile's
+    };
+    while ((ok || MANY) && walk.next(wp)) {  // (with many rows a set that gave up still meets the barrier below)
+      if constexpr (!MANY) {
+        enter(tile_id(0));
+        const int32_t* table = p.block_table + static_cast<int64_t>(walk.seq) * p.bt_stride;
+        for (int g = walk.g; g < walk.g1 && ok; ++g, ++tiles) {
+          if ((tiles & 1) != set) continue;
+          const int key = g * GK + kl, block = wp.block_size.div(key);
+          int32_t page = 0;  // on its way while the scores are made
+          if (key < walk.s.n) page = table[block];
+          float2 sum = make_float2(0.f, 0.f);
+          job(tiles, tiles, g * GK, sum);
+          if (ok && key < walk.s.n) add_weight(wp, page, block, walk.kvh, key, walk.s.vis_base, sum.x + sum.y);
+        }
+      } else {
+        const int kt = tiles_in(walk.g), mine = kt == 2 ? (set - jobs) & 1 : 0;  // this set's tile of the group
+        const int k0 = walk.g * GK + mine * WT_KEYS, key = k0 + kl;
+        const bool writes = kt == 2 || (jobs & 1) == set;  // a lone tile is the set's that has its first job
+        float2 sum = make_float2(0.f, 0.f);
+        for (int qt = walk.qa; qt < walk.qb && ok; ++qt, jobs += kt) {
+          enter(tile_id(qt));
+          const int j = jobs + (kt == 2 ? (set - jobs) & 1 : 0);  // this set's job of the query tile, if it has one
+          if ((j & 1) == set) job(j, tiles + mine, k0, sum);
+        }
+        // whole groups go to the weights, parts of one to the workspace
+        const bool head = walk.qa > walk.first, tail = walk.qb < walk.end;
+        float w = sum.x + sum.y;
+        if (kt == 1) {  // both sets had jobs of the tile
+          if (!writes) red[kl] = w;
+          if (named_bar_or(1, 256, !ok)) break;
+          if (writes) w += red[kl];
+          named_bar_or(1, 256, false);  // read before the next lone tile's
+        }
+        if (ok && writes && key < walk.s.n) {
+          if (head || tail) {
+            wp.part[(static_cast<int64_t>(blockIdx.x) * 2 + (head ? 0 : 1)) * 256 + mine * WT_KEYS + kl] = w;
+          } else {
+            const int block = wp.block_size.div(key);
+            add_weight(wp, p.block_table[static_cast<int64_t>(walk.seq) * p.bt_stride + block], block, walk.kvh, key,
+                       walk.s.vis_base, w);
+          }
+        }
+        if (head) rec_head = make_int4(1, tail, 0, 0);
+        else if (tail) rec_tail = make_int4(1, walk.seq, walk.kvh, walk.g);
+        tiles += kt;
       }
-      if (ok && writes && key < walk.s.n) {
-        if (head || tail)
-          wp.part[(static_cast<int64_t>(blockIdx.x) * 2 + (head ? 0 : 1)) * 256 + mine * WT_KEYS + kl] = w;
-        else add_weight(wp, page, block, walk.kvh, key, walk.s.vis_base, w);
-      }
-      if (head) rec_head = make_int4(1, tail, 0, 0);
-      else if (tail) rec_tail = make_int4(1, walk.seq, walk.kvh, walk.g);
     }
     if (MANY && warp == W::W_SUM && lane == 0) {
       wp.records[2 * blockIdx.x] = rec_head;
@@ -757,51 +824,43 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
       const int idx = e * 32 + lane, key = idx / W::PIECES;
       at[e] = static_cast<uint32_t>(key << 16 | (key * CL::BYTES + (idx - key * W::PIECES) * 8));
     }
-    // lane r < 8 reads the page of run r of the warp's next tile while the present one is copied
-    int t = 0, kt = 0, next = -1;  // next: the tile last looked at
-    int k_next = 0, kvh_next = 0, keys_next = 0;
-    int32_t page_next = 0;
-    const auto look = [&]() {  // on to the warp's next tile; keys_next 0 at the end
-      keys_next = 0;
-      do {
-        if (t == kt) {
-          t = 0;
-          kt = walk.next(wp) ? tiles_in() : 0;
-          if (kt == 0) return;
-        }
-        ++t;
-        ++next;
-      } while (next % W::LOADERS != me);
-      const int k0 = walk.g * GK + (t - 1) * WT_KEYS;
-      k_next = k0 + 16 * (lane & 7);
-      kvh_next = walk.kvh;
-      keys_next = min(WT_KEYS, walk.s.n - k0);
-      if (k_next < walk.s.n)
-        page_next = p.block_table[static_cast<int64_t>(walk.seq) * p.bt_stride + wp.block_size.div(k_next)];
-    };
-    look();
-    while (keys_next > 0) {
-      const int tile = next, st = tile % RS, have = keys_next;
-      const uint8_t* const src =
-          p.cache + page_next * p.block_stride + kvh_next * p.head_stride +
-          static_cast<int64_t>(k_next - wp.block_size.div(k_next) * wp.block_size.d) * CL::BYTES;
-      look();
-      if (tile >= RS) ok = !__any_sync(0xffffffffu, !mbar_wait_spin(&bars[T_RAW_EMPTY + st], (tile / RS - 1) & 1));
-      if (!ok) break;
-      const uint32_t dst = smem_u32(smem + W::OFF_RAW + st * W::STAGE) + lane * 8;
+    int tile = 0;
+    while (ok && walk.next(wp)) {
+      const int32_t* table = p.block_table + static_cast<int64_t>(walk.seq) * p.bt_stride;
+      const uint8_t* head_base = p.cache + walk.kvh * p.head_stride;
+      const int tiles = MANY ? tiles_in(walk.g) : walk.g1 - walk.g, k0 = walk.g * GK;
+      // lane r < 8 reads the page of run r of the warp's next tile while the present one is copied
+      const auto first_key = [&](int t) { return k0 + t * WT_KEYS + 16 * (lane & 7); };
+      const auto page_of = [&](int t) {
+        const int k = first_key(t);
+        return t < tiles && k < walk.s.n ? table[wp.block_size.div(k)] : 0;
+      };
+      int t = (me - tile % W::LOADERS + W::LOADERS) % W::LOADERS;
+      int32_t page = page_of(t);
+      for (; t < tiles && ok; t += W::LOADERS) {
+        const int k = first_key(t), i = tile + t, st = i % RS;
+        const uint8_t* const src = head_base + page * p.block_stride +
+                                   static_cast<int64_t>(k - wp.block_size.div(k) * wp.block_size.d) * CL::BYTES;
+        page = page_of(t + W::LOADERS);
+        if (i >= RS) wait(T_RAW_EMPTY + st, (i / RS - 1) & 1);
+        if (!ok) break;
+        const uint32_t dst = smem_u32(smem + W::OFF_RAW + st * W::STAGE) + lane * 8;
+        const int have = walk.s.n - (k0 + t * WT_KEYS);
 #pragma unroll 1
-      for (int r = 0; r < 8; ++r) {
-        const uint8_t* base = reinterpret_cast<const uint8_t*>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
-        const int keys_r = min(have - 16 * r, 16);  // a run past the sequence is not there
-        if (keys_r <= 0) break;
+        for (int r = 0; r < 8; ++r) {
+          const uint8_t* base = reinterpret_cast<const uint8_t*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
+          const int keys_r = min(have - 16 * r, 16);  // a run past the sequence is not there
+          if (keys_r <= 0) break;
 #pragma unroll
-        for (int e = 0; e < W::RUN_STEPS; ++e)
-          if (static_cast<int>(at[e] >> 16) < keys_r)
-            cp_async8(dst + r * 16 * W::KEY + e * 256, base + (at[e] & 0xFFFFu));
+          for (int e = 0; e < W::RUN_STEPS; ++e)
+            if (static_cast<int>(at[e] >> 16) < keys_r)
+              cp_async8(dst + r * 16 * W::KEY + e * 256, base + (at[e] & 0xFFFFu));
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[T_RAW_FULL + st]))
+                     : "memory");
       }
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[T_RAW_FULL + st]))
-                   : "memory");
+      tile += tiles;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
