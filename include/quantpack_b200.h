@@ -232,6 +232,11 @@ int qp_merge_attn_partials(int dtype, int head_size, int64_t num_tokens, int num
                            int64_t out_stride_token, int64_t out_stride_head, float* lse_out,
                            const uint32_t* rht_sign_bits, void* stream);
 
+/* An entry point by number with its arguments as 64-bit words, in their order: integers and pointers as they are,
+ * floats as the bits of a double. 0: qp_paged_decode, 1: qp_accumulate_attn_weights, 2: qp_evict_cache; `count` is
+ * their argument count (QP_ERR_INVALID otherwise). For bindings that pay for every argument. */
+int qp_invoke(int entry, const void* words, int count);
+
 /* Bytes of workspace qp_accumulate_attn_weights needs. */
 int64_t qp_attn_weights_workspace_bytes(int64_t num_q_tokens, int num_seqs, int max_seqlen_q, int num_q_heads,
                                         int num_kv_heads, int head_size);

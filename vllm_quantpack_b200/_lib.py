@@ -4,6 +4,7 @@ There is no fallback: if the library is missing or does not load, every op raise
 `python -m vllm_quantpack_b200.build` (nvcc, sm_100a)."""
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -37,6 +38,7 @@ SIGNATURES = {
     "qp_prefill_varlen_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
     "qp_prefill_varlen": (_I, [_I, _I, _P, _L, _L, _P, _L, _L, _L, _I, _P, _P, _I, _P, _L, _P, _I, _L, _L, _L, _L, _L,
                                _L, _L, _I, _I, _I, _F, _P, _I, _I, _F, _P, _I, _P, _P, _L, _P]),
+    "qp_invoke": (_I, [_I, ctypes.c_char_p, _I]),
     "qp_attn_weights_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
     "qp_accumulate_attn_weights": (_I, [_I, _I, _P, _L, _L, _L, _I, _P, _P, _I, _I, _P, _L, _P, _I, _L, _L, _L, _L,
                                         _L, _L, _L, _I, _I, _I, _F, _P, _I, _I, _I, _F, _P, _P, _L, _L, _L, _P, _L,
@@ -49,6 +51,12 @@ SIGNATURES = {
     "qp_fold_peer_partials": (_I, [_I, _I, _L, _I, _I, _I, _P, ctypes.c_uint32, _I, _P, _L, _L, _P, _P, _P]),
     "qp_merge_attn_partials": (_I, [_I, _I, _L, _I, _I, _P, _L, _L, _L, _P, _L, _L, _L, _I, _P, _L, _L, _P, _P, _P]),
 }
+
+# Entry points called once a layer and step, with some forty arguments: ctypes takes about 0.2 us to convert each, so
+# they go through qp_invoke, which takes them as one block of 64-bit words (name -> (number, format of the block)).
+_CODES = {_P: "q", _L: "q", _I: "q", _F: "d"}
+_PACKED = {name: (i, struct.Struct("=" + "".join(_CODES[t] for t in SIGNATURES[name][1])))
+           for i, name in enumerate(("qp_paged_decode", "qp_accumulate_attn_weights", "qp_evict_cache"))}
 
 _lock = threading.Lock()
 _lib = None
@@ -81,8 +89,13 @@ def load():
 
 def call(name, *args):
     """Call a qp_* entry point; a non-zero return raises QuantpackError with the library's message."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    lib = _lib or load()
+    packed = _PACKED.get(name)
+    if packed is None:
+        rc = getattr(lib, name)(*args)
+    else:  # a null pointer is None
+        block = packed[1].pack(*[0 if a is None else a for a in args] if None in args else args)
+        rc = lib.qp_invoke(packed[0], block, len(args))
     if rc != 0:
         msg = lib.qp_last_error().decode(errors="replace")
         raise QuantpackError(f"{name}: {msg} (code {rc})")

@@ -22,6 +22,10 @@ def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _device_key(device):
+    return device if type(device) is torch.device else torch.device(device)
+
+
 def _sinks_ptr(sinks, nq, mode):
     """Device pointer of fp32 sink logits (one per query head), or None. Sinks count once in a row's softmax, so
     only the model-domain output (mode 0) can take them, never a partial."""
@@ -177,7 +181,7 @@ def workspace(device, nbytes):
     """A per-device scratch buffer for the split-KV partials, grown geometrically and kept for the process. A
     buffer that is outgrown stays allocated too: a CUDA graph captured earlier may still hold its address. Growing
     it inside a CUDA-graph capture allocates from the graph's pool: reserve the largest size before capturing."""
-    key = str(torch.device(device))
+    key = _device_key(device)
     ws = _workspaces.get(key)
     if ws is not None and ws.numel() >= nbytes:  # the common case: no growth, no lock
         return ws
@@ -196,7 +200,7 @@ _sm_counts = {}
 
 
 def sm_count(device):
-    key = str(torch.device(device))
+    key = _device_key(device)
     n = _sm_counts.get(key)
     if n is None:
         n = _sm_counts[key] = torch.cuda.get_device_properties(device).multi_processor_count
@@ -249,27 +253,32 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
     logits whose exp joins every row's softmax denominator (vLLM's attention sinks; model-domain output only).
     lse_out: None or (tokens, query heads) fp32, filled with the base-2 log-sum-exp of each row's scaled scores, sinks
     included (what `accumulate_attention_weights` takes), beside a model-domain output."""
-    hs = q.shape[-1]
-    nq = q.shape[1]
+    tokens, nq, hs = q.shape
+    q_st, q_sh, q_sc = q.stride()
+    out_st, out_sh, out_sc = out.stride()
+    bt_st, bt_sc = block_table.stride()
+    device = q.device
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
     nkv = lay.nkv
     num_seqs = cu_seqlens_q.shape[0] - 1
+    if hs == 128:
+        _check_device(device, key_cache=key_cache, out=out)
     if num_splits is None:
         keys = window_keys(max_seqlen_k, sliding_window, max_seqlen_q)
         if hs == 128:
             num_splits = _memo("qp_decode_num_splits_head", hs, int(max_seqlen_q) * (nq // nkv), num_seqs, nkv, keys,
-                               sm_count(q.device))
+                               sm_count(device))
         else:
-            num_splits = decode_num_splits(num_seqs, nkv, keys, sm_count(q.device))
-    wbytes = _memo("qp_decode_workspace_bytes", int(q.shape[0]), int(nq), int(hs), int(num_splits))
+            num_splits = decode_num_splits(num_seqs, nkv, keys, sm_count(device))
+    wbytes = _memo("qp_decode_workspace_bytes", tokens, nq, hs, int(num_splits))
     if ws is None:
-        ws = workspace(q.device, wbytes)
-    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("seqused_k", seqused_k), ("block_table", block_table)):
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32")
-    if cu_seqlens_q.stride(0) != 1 or seqused_k.stride(0) != 1 or block_table.stride(-1) != 1:
+        ws = workspace(device, wbytes)
+    int32 = torch.int32
+    if cu_seqlens_q.dtype != int32 or seqused_k.dtype != int32 or block_table.dtype != int32:
+        raise TypeError("cu_seqlens_q, seqused_k and block_table must be int32")
+    if cu_seqlens_q.stride(0) != 1 or seqused_k.stride(0) != 1 or bt_sc != 1:
         raise ValueError("cu_seqlens_q, seqused_k and block_table rows must be contiguous")
-    if q.stride(-1) != 1 or out.stride(-1) != 1:
+    if q_sc != 1 or out_sc != 1:
         raise ValueError("q / out rows must be contiguous")
     dt = _dtype_code(q, "paged_decode")
     if partials_only:
@@ -284,13 +293,13 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
         if out.dtype != q.dtype:
             raise TypeError("out dtype must match q")
         mode, lse_ptr = 0, None
-    lse_ptr = _lse_ptr(lse_out, q.shape[0], nq, mode, out_fp32_lse) or lse_ptr
-    _lib.call("qp_paged_decode", lay.fmt, dt, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-              out.stride(1), q.shape[0], num_seqs, cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q),
-              block_table.data_ptr(), block_table.stride(0), *lay.args(), nq, nkv, hs, float(softmax_scale),
-              rht.device_sign_bits(hs, q.device).data_ptr(), int(bool(q_rotated)), int(tokens_after_keys),
-              int(sliding_window), float(softcap or 0.0), _sinks_ptr(sinks, nq, mode), mode, lse_ptr, int(num_splits),
-              ws.data_ptr(), ws.numel() * ws.element_size(), _stream(q.device))
+    if lse_out is not None:
+        lse_ptr = _lse_ptr(lse_out, tokens, nq, mode, out_fp32_lse)
+    _lib.call("qp_paged_decode", lay.fmt, dt, q.data_ptr(), q_st, q_sh, out.data_ptr(), out_st, out_sh, tokens,
+              num_seqs, cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q), block_table.data_ptr(), bt_st,
+              *lay.args(), nq, nkv, hs, float(softmax_scale), rht.device_sign_bits(hs, device).data_ptr(),
+              int(bool(q_rotated)), int(tokens_after_keys), int(sliding_window), float(softcap or 0.0),
+              _sinks_ptr(sinks, nq, mode), mode, lse_ptr, int(num_splits), ws.data_ptr(), ws.nbytes, _stream(device))
     return ws if partials_only else out
 
 
@@ -421,15 +430,16 @@ def new_attention_weights(k_scale_cache):
 
 def _check_device(device, **tensors):
     """The launch goes to the current device: every tensor has to live there."""
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         raise ValueError(f"the tensors are on {device}, the current device is {torch.cuda.current_device()}")
     for name, t in tensors.items():
-        if t.device != device:
+        if t.get_device() != index:
             raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def _check_weights(weights, lay):
-    if weights.dtype != torch.float32 or tuple(weights.shape) != (lay.nblocks, lay.block_size, lay.nkv):
+    if weights.dtype != torch.float32 or weights.shape != (lay.nblocks, lay.block_size, lay.nkv):
         raise ValueError(f"weights must be fp32 (blocks, block size, KV heads) = "
                          f"({lay.nblocks}, {lay.block_size}, {lay.nkv}), got {weights.dtype} {tuple(weights.shape)}")
 
@@ -452,27 +462,28 @@ def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_
     tokens have no earlier weight: theirs is stored, so pages need no clearing before reuse as long as every token
     enters through such a call; a first call that covers only the last tokens of a prompt wants the other cells zeroed.
     Cells past a sequence's length are left as they are. Returns `weights`."""
-    hs, nq = q.shape[-1], q.shape[1]
+    tokens, nq, hs = q.shape
+    q_st, q_sh, q_sc = q.stride()
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
     _check_weights(weights, lay)
     _check_index(cu_seqlens_q=cu_seqlens_q, seqused_k=seqused_k, block_table=block_table)
-    if q.stride(-1) != 1:
+    if q_sc != 1:
         raise ValueError("q rows must be contiguous")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], nq) or not lse.is_contiguous():
-        raise ValueError(f"lse must be contiguous fp32 ({q.shape[0]}, {nq})")
+    if lse.dtype != torch.float32 or lse.shape != (tokens, nq) or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous fp32 ({tokens}, {nq})")
     dt = _dtype_code(q, "accumulate_attention_weights")
     _check_device(q.device, key_cache=key_cache, weights=weights, lse=lse, cu_seqlens_q=cu_seqlens_q,
                   seqused_k=seqused_k, block_table=block_table)
     num_seqs = cu_seqlens_q.shape[0] - 1
     if ws is None:
-        ws = workspace(q.device, _memo("qp_attn_weights_workspace_bytes", int(q.shape[0]), num_seqs,
-                                       int(max_seqlen_q), int(nq), lay.nkv, int(hs)))
-    _lib.call("qp_accumulate_attn_weights", lay.fmt, dt, q.data_ptr(), q.stride(0), q.stride(1), q.shape[0], num_seqs,
+        ws = workspace(q.device, _memo("qp_attn_weights_workspace_bytes", tokens, num_seqs, int(max_seqlen_q), nq,
+                                       lay.nkv, hs))
+    _lib.call("qp_accumulate_attn_weights", lay.fmt, dt, q.data_ptr(), q_st, q_sh, tokens, num_seqs,
               cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q), int(max_seqlen_k),
               block_table.data_ptr(), block_table.stride(0), *lay.args(), nq, lay.nkv, hs, float(softmax_scale),
               rht.device_sign_bits(hs, q.device).data_ptr(), int(bool(q_rotated)), int(tokens_after_keys),
               int(sliding_window), float(softcap or 0.0), lse.data_ptr(), weights.data_ptr(), *weights.stride(),
-              ws.data_ptr(), ws.numel() * ws.element_size(), _stream(q.device))
+              ws.data_ptr(), ws.nbytes, _stream(q.device))
     return weights
 
 
@@ -512,6 +523,6 @@ def evict_cache(key_cache, value_cache, weights, *, seqused_k, max_seqlen_k, blo
               block_table.data_ptr(), block_table.stride(0),
               out_block_table.data_ptr() if out_block_table is not None else None,
               out_block_table.stride(0) if out_block_table is not None else 0, keep, int(keep_first), int(keep_last),
-              kept.data_ptr(), seqused_out.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(),
+              kept.data_ptr(), seqused_out.data_ptr(), ws.data_ptr(), ws.nbytes,
               _stream(key_cache.device))
     return kept, seqused_out

@@ -41,7 +41,7 @@ def device_sign_bits(head_size, device):
     """The sign words as an int32 tensor on `device` (cached; the first call per device copies from the host, so make
     it before any CUDA-graph capture)."""
     import torch
-    key = (head_size, str(torch.device(device)))
+    key = (head_size, device if type(device) is torch.device else torch.device(device))
     t = _device_bits.get(key)
     if t is None:
         t = torch.from_numpy(sign_bits(head_size).view(np.int32).copy()).to(device)

@@ -3,6 +3,9 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <tuple>
+#include <type_traits>
+
 #include "qp_api_internal.h"
 #include "qp_common.cuh"
 
@@ -51,4 +54,52 @@ extern "C" int qp_device_error(int* code) {
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(qp::g_device_error, &zero, sizeof(int));
   if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "qp_device_error: %s", cudaGetErrorString(e));
   return QP_OK;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The entry points with the longest argument lists, from a block of 64-bit words.
+#include "../../include/quantpack_b200.h"
+
+namespace {
+struct Words {
+  const char* at;
+  template <class T>
+  T take() {
+    if constexpr (std::is_same<T, float>::value) {
+      double v;
+      memcpy(&v, at, 8);
+      at += 8;
+      return static_cast<float>(v);
+    } else {
+      int64_t v;
+      memcpy(&v, at, 8);
+      at += 8;
+      if constexpr (std::is_pointer<T>::value) return reinterpret_cast<T>(static_cast<uintptr_t>(v));
+      else return static_cast<T>(v);
+    }
+  }
+};
+
+// braces: the words are taken in the order of the parameters
+template <class... A>
+struct Call {
+  std::tuple<A...> args;
+  explicit Call(Words w) : args{w.take<A>()...} {}
+};
+template <class... A>
+int invoke(int (*fn)(A...), const void* words, int count) {
+  if (count != static_cast<int>(sizeof...(A)))
+    return set_error(QP_ERR_INVALID, "invoke: %d arguments, expected %d", count, static_cast<int>(sizeof...(A)));
+  return std::apply(fn, Call<A...>(Words{static_cast<const char*>(words)}).args);
+}
+}  // namespace
+
+extern "C" int qp_invoke(int entry, const void* words, int count) {
+  if (!words) return set_error(QP_ERR_INVALID, "invoke: null pointer");
+  switch (entry) {
+    case 0: return invoke(qp_paged_decode, words, count);
+    case 1: return invoke(qp_accumulate_attn_weights, words, count);
+    case 2: return invoke(qp_evict_cache, words, count);
+    default: return set_error(QP_ERR_INVALID, "invoke: entry %d", entry);
+  }
 }
