@@ -79,8 +79,8 @@ __device__ __forceinline__ void add_cluster(void* p, uint32_t rank, uint32_t v) 
 constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048;
 
 struct EvictShared {
-  uint32_t hist[EV_BINS];   // this CTA's
-  uint32_t total[EV_BINS];  // in the first CTA: the cluster's
+  uint32_t hist[EV_BINS];      // this CTA's
+  uint32_t total[3][EV_BINS];  // in the first CTA: the cluster's, one for each digit
   uint32_t bin, left;      // the digit found, and how many of its weights stay
   uint32_t warp_sum[EV_WARPS];
   uint32_t gt[EV_WARPS], tie[EV_WARPS];  // per warp: tokens that stay for sure, tokens at the threshold
@@ -120,17 +120,19 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     const int k = i - c0;
     return k < p.smem_weights ? ranks[k] : weight_rank(*weight_at(p, table, kvh, i));
   };
+  for (int i = tid; i < 3 * EV_BINS; i += EV_THREADS) (&sh.total[0][0])[i] = 0;
 #pragma unroll 8
   for (int i = c0 + tid; i < min(c1, c0 + p.smem_weights); i += EV_THREADS)
     ranks[i - c0] = weight_rank(*weight_at(p, table, kvh, i));
 
+  sync();  // the first CTA's totals are zero before anyone adds to them
   uint32_t thr = 0, mask = 0, want = p.keep - p.first - p.last;  // of the tokens [lo, hi)
   const int b0 = max(c0, lo), b1 = min(c1, hi);
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : EV_BINS;
-    for (int i = tid; i < EV_BINS; i += EV_THREADS) sh.hist[i] = sh.total[i] = 0;
-    sync();
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) sh.hist[i] = 0;
+    __syncthreads();
     for (int i = b0 + tid; i < b1; i += EV_THREADS) {
       const uint32_t r = rank_of(i);
       if ((r & mask) == thr) atomicAdd(&sh.hist[(r >> shift) & (bins - 1)], 1u);
@@ -138,13 +140,13 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     __syncthreads();
     for (int i = tid; i < EV_BINS; i += EV_THREADS)  // few bins hold anything
       if (sh.hist[i] != 0u) {
-        if (rank == 0) atomicAdd(&sh.total[i], sh.hist[i]);
-        else add_cluster(&sh.total[i], 0, sh.hist[i]);
+        if (rank == 0) atomicAdd(&sh.total[pass][i], sh.hist[i]);
+        else add_cluster(&sh.total[pass][i], 0, sh.hist[i]);
       }
     sync();
     if (rank == 0) {  // the bin in which the want-th heaviest lies, from the highest on (2 bins a thread)
       const int top = EV_BINS - 1 - 2 * tid;
-      const uint32_t h0 = sh.total[top], h1 = sh.total[top - 1];
+      const uint32_t h0 = sh.total[pass][top], h1 = sh.total[pass][top - 1];
       uint32_t incl = h0 + h1;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(MV_THREADS, MV_CTAS) evict_move_kernel(const E
 }
 
 // CTAs of a pair's cluster: about EV_PART tokens each, 16 at most
-constexpr int EV_PART = 16384;
+constexpr int EV_PART = 16384, EV_HELD = 46 * 1024;
 static int evict_cluster(int max_n) {
   int c = 1;
   while (c < 16 && c * EV_PART < max_n) c *= 2;
@@ -399,7 +401,7 @@ extern "C" int qp_evict_cache(void* cache, int cell_bytes, int block_size, int64
   if (tickets > 0x7fffffff) return set_error(QP_ERR_UNSUPPORTED, "evict: grid too large");
   const int cluster = evict_cluster(max_seqlen_k);
   const int part = (max_seqlen_k + cluster - 1) / cluster;
-  const int held = std::min(part, 48 * 1024);
+  const int held = std::min(part, EV_HELD);
   int2* lens = static_cast<int2*>(workspace);
   uint32_t* ticket = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + (num_seqs * 8ll + 15) / 16 * 16);
   const EvictParams p{static_cast<uint8_t*>(cache), FastDiv(block_size), block_stride, head_stride, slot_stride,
@@ -412,7 +414,7 @@ extern "C" int qp_evict_cache(void* cache, int cell_bytes, int block_size, int64
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
     cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(sizeof(EvictShared)) + 48 * 1024 * 4);
+                                         static_cast<int>(sizeof(EvictShared)) + EV_HELD * 4);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return set_error(QP_ERR_CUDA, "evict attribute: %s", cudaGetErrorString(e));

@@ -611,13 +611,15 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
       tc_fence_after();
       if (elect_one()) {
         const uint32_t ak = tmem + sl * W::ACOLS, sd = tmem + W::S + buf * NR;
+        // the small term first: each accumulation rounds the sum so far toward zero, and so only the HS / 16 of the
+        // large term meet a large sum (the other order: errors of the weights 2 to 3 times as large)
 #pragma unroll
-        for (int term = 0; term < 2; ++term)
+        for (int term = 1; term >= 0; --term)
 #pragma unroll
           for (int c = 0; c < HS / 16; ++c)
             umma_f16_ts(sd, ak + 8 * c,
                         qd + static_cast<uint64_t>((term * W::TERM + (c >> 2) * W::ATOM + (c & 3) * 32) >> 4), ID,
-                        (term | c) ? 1u : 0u);
+                        (term == 0 || c > 0) ? 1u : 0u);
         umma_commit(&bars[T_S_FULL + buf]);
       }
       __syncwarp();
