@@ -284,3 +284,38 @@ def test_static_scratch_graph_and_stream(device):
         decode(other)
     side.synchronize()
     assert torch.equal(other, captured)
+
+
+@pytest.mark.parametrize("varlen", [False, True])
+def test_rows_behind_the_last_sequence_stay(device, varlen):
+    """A batch padded to a captured size: rows no sequence owns keep what they held, the output's and the lse's."""
+    lens, qlens, nq, pad = [300, 40], [2, 1], 16, 5
+    cache, table = setup(device, "int4", lens, seed=11)
+    qb = U.make_queries([3 + pad], seed=17, nq=nq, hs=HS)
+    q = U.to_torch(qb, device)
+    kc, vc, ks, vs = cache.views
+    out = torch.full_like(q, 3.0)
+    lse = torch.full((3 + pad, nq), 5.0, dtype=torch.float32, device=device)
+    args = dict(cu_seqlens_q=torch.tensor([0, 2, 3], dtype=torch.int32, device=device),
+                seqused_k=torch.tensor(lens, dtype=torch.int32, device=device), max_seqlen_k=300,
+                softmax_scale=HS ** -0.5, block_table=torch.from_numpy(table).to(device), k_scale_cache=ks,
+                v_scale_cache=vs, lse_out=lse)
+    if varlen:
+        ops.prefill_varlen(q, kc, vc, out, **args)
+    else:
+        ops.paged_decode(q, kc, vc, out, max_seqlen_q=2, **args)
+    assert (out[3:] == 3.0).all() and (lse[3:] == 5.0).all()
+    check(cache, table, qb[:3], qlens, lens, out[:3].float().cpu().numpy())
+
+
+def test_many_short_sequences_and_every_row_finite(device):
+    """More (sequence, KV head) pairs than CTAs, most of them shorter than a tile: shares that cross many pairs."""
+    rng = np.random.default_rng(12)
+    lens = [int(n) for n in rng.integers(1, 90, 150)] + [3000]
+    qlens = [min(4, n) for n in lens]
+    cache, table = setup(device, "k8v4", lens, seed=12)
+    qb = U.make_queries(qlens, seed=18, nq=8, hs=HS)
+    for splits in (None, 2, 40):
+        got = U.decode(cache, qb, qlens, lens, table, num_splits=splits)
+        assert np.isfinite(got).all()
+        check(cache, table, qb, qlens, lens, got)

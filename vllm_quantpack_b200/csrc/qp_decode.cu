@@ -1366,9 +1366,10 @@ extern "C" int qp_paged_decode(int fmt, int dtype, const void* q, int64_t q_stri
   rc = launch_decode(fmt, dtype, head_size, dp, max_seqlen_q * group, num_seqs, st);
   if (rc) return rc;
   if (out_mode == 2) return QP_OK;  // split partials stay in the workspace
-  return merge_dispatch(decode_merge_params(dp, head_size, out_mode, out, out_stride_token, out_stride_head, lse_out,
-                                          sinks),
-                        dtype, head_size, num_q_tokens, st, true);
+  MergeParams mp = decode_merge_params(dp, head_size, out_mode, out, out_stride_token, out_stride_head, lse_out, sinks);
+  mp.cu_seqlens_q = cu_seqlens_q;
+  mp.num_seqs = num_seqs;
+  return merge_dispatch(mp, dtype, head_size, num_q_tokens, st, true);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1565,9 +1566,10 @@ extern "C" int qp_prefill_varlen(int fmt, int dtype, const void* q, int64_t q_st
   decode_bind_workspace(dp, workspace, head_size);
   rc = launch_decode(fmt, dtype, head_size, dp, cq * group, upper, st);
   if (rc) return rc;
-  return merge_dispatch(decode_merge_params(dp, head_size, out_mode, out, out_stride_token, out_stride_head, lse_out,
-                                          sinks),
-                        dtype, head_size, num_q_tokens, st, true);
+  MergeParams mp = decode_merge_params(dp, head_size, out_mode, out, out_stride_token, out_stride_head, lse_out, sinks);
+  mp.cu_seqlens_q = cu_seqlens_q;
+  mp.num_seqs = num_chunks;
+  return merge_dispatch(mp, dtype, head_size, num_q_tokens, st, true);
 }
 
 // ---------------------------------------------------------------------------------------------------------------

@@ -126,6 +126,10 @@ struct MergeParams {
   // denominator once, vLLM's attention sinks (vllm/v1/attention/ops/triton_attention_helpers.py:108-138: the row
   // maximum starts at the sink with sum 1 in one segment only; triton_unified_attention.py:356-359)
   const float* sinks;
+  // head 128, may be null: rows outside the query tokens [cu_seqlens_q[0], cu_seqlens_q[num_seqs]) are left alone (a
+  // padded batch: nothing wrote their partials)
+  const int32_t* cu_seqlens_q;
+  int num_seqs;
 };
 
 // Launches the head-128 kernel (qp_decode128.cu) on the parameters of launch_decode, `rows` query rows per KV head at

@@ -45,6 +45,7 @@ struct D1 {
   static constexpr int CTAS = NT == 1 ? 2 : 1;  // per SM: 128 registers a thread, or 168 / 255
   static constexpr int THREADS = 32 * WARPS;
   static constexpr int ROWS = 8 * NT;
+  static constexpr int START = NT == 1 ? 32 : 64;  // what starting on a pair costs, in tiles (find_share)
   static constexpr int RUNS = NT <= 2 ? 2 : 1;  // 16-key runs taken at a time (registers)
   static constexpr int STAGE = D1_KEYS * CL::BYTES;
   static constexpr int STAGES = FMT == FMT_INT4 ? (NT >= 3 ? 4 : 3) : (NT >= 3 ? 3 : 2);
@@ -144,13 +145,13 @@ __device__ __forceinline__ void close_slots(const DecodeParams& p, const DecodeS
 }
 
 // A balanced launch: the tiles of all (sequence, KV head) pairs in a row, sequence by sequence, head by head, each pair
-// led by D1_START units that stand for what starting on it costs a CTA (its query rows, the first copies' latency, the
-// merge of the warps: measured near 3 us, 4 tiles a warp), cut into shares of `share` units; CTA c takes the c-th. The
+// led by C::START units that stand for what starting on it costs a CTA (its query rows, the first copies' latency, the
+// merge of the warps), cut into shares of `share` units; CTA c takes the c-th. Measured (us; START 32 / 64 / 128): 12
+// rows over 131,072 keys 39.0 / 35.0 / 35.4, a ragged k8v4 batch of 16 rows 81.4 / 75.4 / 79.9, 8 rows over 1000 keys
+// 12.4 / 14.4 / 14.4; without it, CTAs that meet two pairs end last (n 131,072: 45). The
 // shares with tiles of a pair are its partials, in order. share: as even as the grid allows, at least a tile a warp,
 // and so long that no pair meets more than num_splits shares (T <= share (num_splits - 1) tiles meet at most
 // num_splits).
-constexpr int D1_START = 32;
-
 struct Share {
   int64_t share, hi;  // units of a share, end of this CTA's
   int64_t unit;       // where the pair of (seq, kvh) starts
@@ -165,7 +166,7 @@ __device__ __forceinline__ bool find_share(const DecodeParams& p, uint8_t* smem,
   int64_t* found = reinterpret_cast<int64_t*>(smem);  // sequence, its first unit, its tiles
   int64_t* tot = found + 4;                           // [WARPS]
   int* top = reinterpret_cast<int*>(tot + C::WARPS);  // [WARPS]
-  const auto units_of = [&](int t) { return t > 0 ? static_cast<int64_t>(t + D1_START) * p.nkv : 0; };
+  const auto units_of = [&](int t) { return t > 0 ? static_cast<int64_t>(t + C::START) * p.nkv : 0; };
   int64_t total = 0;
   int most = 0, mine = 0;
   for (int b = tid; b < p.num_seqs; b += C::THREADS) {
@@ -196,7 +197,7 @@ __device__ __forceinline__ bool find_share(const DecodeParams& p, uint8_t* smem,
   }
   // (shares of under 2^31 units: a cache of 2^36 keys)
   const uint32_t even = static_cast<uint32_t>((total + ctas - 1) / ctas);
-  const uint32_t room = static_cast<uint32_t>(most + D1_START + p.num_splits - 2) / (p.num_splits - 1);
+  const uint32_t room = static_cast<uint32_t>(most + C::START + p.num_splits - 2) / (p.num_splits - 1);
   const int64_t share = max(max(even, room), static_cast<uint32_t>(C::WARPS));
   const int64_t lo = cta * share, hi = min(lo + share, total);
   if (lo >= hi) return false;
@@ -231,8 +232,8 @@ __device__ __forceinline__ bool find_share(const DecodeParams& p, uint8_t* smem,
   __syncthreads();
   out.seq = static_cast<int>(found[0]);
   out.tiles = static_cast<int>(found[2]);
-  out.kvh = static_cast<int>(static_cast<uint32_t>(lo - found[1]) / static_cast<uint32_t>(out.tiles + D1_START));
-  out.unit = found[1] + static_cast<int64_t>(out.kvh) * (out.tiles + D1_START);
+  out.kvh = static_cast<int>(static_cast<uint32_t>(lo - found[1]) / static_cast<uint32_t>(out.tiles + C::START));
+  out.unit = found[1] + static_cast<int64_t>(out.kvh) * (out.tiles + C::START);
   out.share = share;
   out.hi = hi;
   __syncthreads();
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__((D1<FMT, NT>::THREADS), (D1<FMT, NT>::CTAS)) d
     const int tile_lo = FEAT ? first_tile(p, sp) : 0;
     int at, ntl, close = slot + 1;  // the partials [slot + 1, close) get no keys
     if (p.balanced) {
-      const int64_t first = sh.unit + D1_START;  // unit of the pair's tile 0
+      const int64_t first = sh.unit + C::START;  // unit of the pair's tile 0
       const int64_t lo = max(blockIdx.x * sh.share, first), hi = min(sh.hi, first + sh.tiles);
       at = static_cast<int>(lo - first);
       ntl = static_cast<int>(hi - lo);  // 0 or less: the share ends inside the pair's lead
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__((D1<FMT, NT>::THREADS), (D1<FMT, NT>::CTAS)) d
       close_slots(p, sp, kvh, rows, slot + 1, close, tid, C::THREADS);
     }
     if (!p.balanced) return;
-    sh.unit += D1_START + sh.tiles;  // on to the next pair
+    sh.unit += C::START + sh.tiles;  // on to the next pair
     if (sh.unit >= sh.hi) return;
     if (++kvh == p.nkv) {
       kvh = 0;
@@ -777,6 +778,7 @@ __global__ void __launch_bounds__(32 * MG_WARPS) merge128_kernel(const MergePara
   if (r >= rows) return;  // only where a warp is a row
   const int64_t tok = r / p.nq;
   const int qh = static_cast<int>(r % p.nq);
+  if (p.cu_seqlens_q != nullptr && (tok < p.cu_seqlens_q[0] || tok >= p.cu_seqlens_q[p.num_seqs])) return;
   const float* lse = p.part_lse + tok * p.pl_t + qh * p.pl_h;
   float w[NC], M = -INFINITY;
 #pragma unroll
