@@ -461,7 +461,8 @@ def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_
     `lse_out`. Summed over the query tokens (one, or a whole prompt) and the query heads of each KV head. The call's own
     tokens have no earlier weight: theirs is stored, so pages need no clearing before reuse as long as every token
     enters through such a call; a first call that covers only the last tokens of a prompt wants the other cells zeroed.
-    Cells past a sequence's length are left as they are. Returns `weights`."""
+    Cells past a sequence's length are left as they are. Calls that overlap on the GPU (two streams, two graphs replayed
+    at once) need workspaces of their own (`ws`). Returns `weights`."""
     tokens, nq, hs = q.shape
     q_st, q_sh, q_sc = q.stride()
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
@@ -495,7 +496,8 @@ def evict_cache(key_cache, value_cache, weights, *, seqused_k, max_seqlen_k, blo
     sequence stays a sequence of min(length, keep) tokens for every call that reads it. In place (no other sequence may
     hold the pages), or with `out_block_table` (int32 (seqs, pages)) into other pages, the old ones left as they are: a
     sequence whose pages others share (a common prompt). Returns (kept, seqused): the old positions (seqs, KV heads,
-    keep) int32, -1 behind the last, and the new lengths (`seqused_out` if given, which may be `seqused_k` itself)."""
+    keep) int32, -1 behind the last, and the new lengths (`seqused_out` if given, which may be `seqused_k` itself).
+    Calls that overlap on the GPU need workspaces of their own (`ws`)."""
     int4 = key_cache.dtype == torch.uint8
     hs = (key_cache.shape[-1] - 4) * 2 if int4 else key_cache.shape[-1]
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
