@@ -298,3 +298,23 @@ def test_score_evict_attend(device, fmt, hs, nq, nkv):
             o = p @ np.asarray(V, np.float64)[idx, h] / p.sum(-1, keepdims=True)
             want[b, h * group:(h + 1) * group] = qo.single_rht(o.astype(np.float32), sg, inverse=True) / hs
     assert qo.relerr(out.float().cpu().numpy(), want) < 5e-3
+
+
+@pytest.mark.parametrize("fmt,qlens,lens", [("k8v4", [150], [700]), ("int4", [3] * 40, list(range(3, 363, 9)))])
+def test_query_records_change_hands(device, fmt, qlens, lens):
+    """Head 512, where the ring holds one query record: it is copied over as soon as the summing warps have given the
+    one before back, in the middle of masked tiles (a window, causal ends). A key's sum has a fixed order, so twenty
+    calls give the same bits, within the bound of the definition."""
+    cache, table = setup(device, fmt, 512, lens, nkv=1, seed=31)
+    qb = U.make_queries(qlens, seed=32, nq=8, hs=512)
+    before = start_weights(cache, device)
+    want, lse, rtol, added = expect(cache, table, qb, qlens, lens, before, window=100)
+    lse = torch.from_numpy(lse).to(device)
+    first = None
+    for _ in range(20):
+        got = run(device, cache, table, qb, qlens, lens, before.clone(), lse, sliding_window=100)
+        if first is None:
+            first = got
+            err = np.abs(got.cpu().numpy() - want)
+            assert (err <= rtol * added + 2.0 ** -23 * np.abs(want) + 1e-37).all()
+        assert torch.equal(got, first)

@@ -714,6 +714,7 @@ __global__ void __launch_bounds__((WT<FMT, HS, NR, KT, MANY>::THREADS), 1) weigh
     const auto enter = [&](int64_t id) {
       if (id == cur) return;
       cur = id;
+      __syncwarp();  // the lanes read the record's rows past the score buffer's hand-off, each at its own pace
       if (loads > 0 && lane == 0) mbar_arrive(&bars[T_Q_EMPTY + (loads - 1) % QS]);
       wait(T_Q_FULL + loads % QS, (loads / QS) & 1);
       rec = smem + (loads % QS) * W::QREC;
