@@ -318,3 +318,22 @@ def test_query_records_change_hands(device, fmt, qlens, lens):
             err = np.abs(got.cpu().numpy() - want)
             assert (err <= rtol * added + 2.0 ** -23 * np.abs(want) + 1e-37).all()
         assert torch.equal(got, first)
+
+
+@pytest.mark.parametrize("fmt,hs", [("int4", 128), ("k8v4", 256)])
+def test_long_prompt_of_alike_weights(device, fmt, hs):
+    """A prompt of 16,384 tokens whose rows give every key they see the same weight (zero queries, one lse): up to
+    131,072 equal additions a key, whose roundings all fall the same way where they are added one by one.
+
+    Bound, relative, whatever the rows: the exponential 2^-22; a tile of 64 rows is added up in two chains of 32, 31 x
+    2^-24 (half a step each); the sum over the tiles is compensated, 2 x 2^-24; the two chains 2^-24; the parts of a group
+    that several CTAs share are added in 64 bits, 2^-24 for the result."""
+    n, nq, lse_value = 16384, 8, np.float32(1.7)
+    cache, table = setup(device, fmt, hs, [n], nkv=1, seed=41)
+    q = torch.zeros((n, nq, hs), dtype=torch.bfloat16, device=device)
+    lse = torch.full((n, nq), float(lse_value), device=device)
+    got = run(device, cache, table, None, [n], [n], start_weights(cache, device), lse, q=q)
+    got = got.cpu().numpy()[table[0]].reshape(-1)[:n]
+    want = nq * (n - np.arange(n, dtype=np.float64)) * np.exp2(-np.float64(lse_value))
+    rel = np.abs(got / want - 1)
+    assert rel.max() <= 2.0 ** -22 + (31 + 2 + 1 + 1) * 2.0 ** -24, rel.max()
