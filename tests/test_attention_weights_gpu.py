@@ -337,3 +337,22 @@ def test_long_prompt_of_alike_weights(device, fmt, hs):
     want = nq * (n - np.arange(n, dtype=np.float64)) * np.exp2(-np.float64(lse_value))
     rel = np.abs(got / want - 1)
     assert rel.max() <= 2.0 ** -22 + (31 + 2 + 1 + 1) * 2.0 ** -24, rel.max()
+
+
+@pytest.mark.parametrize("fmt,hs", [("int4", 128), ("k8v4", 256), ("int4", 512)])
+@pytest.mark.parametrize("qlen", [1, 30])
+def test_nan_in_cells_no_row_sees(device, fmt, hs, qlen):
+    """Cells in front of every row's window hold NaN scales (their pages may be another's by now): they get nothing,
+    and the tile's other keys what is theirs."""
+    n, window = 903, 77
+    cache, table = setup(device, fmt, hs, [n], nkv=2, seed=43)
+    qb = U.make_queries([qlen], seed=44, nq=6, hs=hs)
+    before = start_weights(cache, device)
+    want, lse, rtol, added = expect(cache, table, qb, [qlen], [n], before, window=window)
+    raw = cache.phys.view(torch.uint8)
+    for i in range(n - qlen + 1 - window):
+        raw[int(table[0][i // 16]), :, i % 16] = 0xFF
+    got = run(device, cache, table, qb, [qlen], [n], before.clone(), torch.from_numpy(lse).to(device),
+              sliding_window=window).cpu().numpy()
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= rtol * added + 2.0 ** -23 * np.abs(want) + 1e-37).all()

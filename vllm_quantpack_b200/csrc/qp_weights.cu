@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(256) weights_qprep_kernel(const WeightParams w
   if (lane < RW) {  // this lane's row of the warp: its bounds and -lse
     const int rt = warp * RW + lane, r = qt * NR + rt;
     float nl = -INFINITY;
-    int vis = INT_MAX, lo = INT_MIN;
+    int vis = INT_MIN, lo = INT_MIN;  // a padding row sees no key: where a tile is masked it adds 0, whatever a cell holds
     if (r < rows) {
       const int tok = r / p.group;
       const float l = wp.lse[static_cast<int64_t>(q0 + tok) * p.nq + kvh * p.group + r % p.group];
