@@ -319,3 +319,32 @@ def test_many_short_sequences_and_every_row_finite(device):
         got = U.decode(cache, qb, qlens, lens, table, num_splits=splits)
         assert np.isfinite(got).all()
         check(cache, table, qb, qlens, lens, got)
+
+
+def spoil(cache, table_row, positions):
+    """NaN scales and codes of all ones in the cells of these positions."""
+    raw = cache.phys.view(torch.uint8)
+    for i in positions:
+        raw[int(table_row[i // cache.block_size]), :, i % cache.block_size] = 0xFF
+
+
+@pytest.mark.parametrize("fmt", ["int4", "k8v4"])
+@pytest.mark.parametrize("splits", [None, 1])
+def test_nan_in_cells_a_row_does_not_see(device, fmt, splits):
+    """Cells in front of a sliding window (their pages may be another's by now) and the newest token's cell, which the
+    earlier query tokens do not see, hold NaN: they reach no row that does not see them."""
+    n, window, nq = 2101, 40, 16
+    for qlen in (1, 3):
+        cache, table = setup(device, fmt, [n], seed=52)
+        qb = U.make_queries([qlen], seed=53, nq=nq, hs=HS)
+        want = U.reference(cache.host_bytes(), cache.layout, qb, [qlen], [n], table, sliding_window=window)
+        spoil(cache, table[0], range(n - qlen + 1 - window))
+        got = U.decode(cache, qb, [qlen], [n], table, num_splits=splits, sliding_window=window)
+        assert qo.relerr(got, want) < TOL
+    cache, table = setup(device, fmt, [n], seed=54)
+    qb = U.make_queries([4], seed=55, nq=nq, hs=HS)
+    want = U.reference(cache.host_bytes(), cache.layout, qb, [4], [n], table)
+    spoil(cache, table[0], [n - 1])
+    got = U.decode(cache, qb, [4], [n], table, num_splits=splits)
+    assert qo.relerr(got[:3], want[:3]) < TOL
+    assert np.isnan(got[3]).all()

@@ -442,6 +442,7 @@ __device__ __forceinline__ bool decode128_segment(const DecodeParams& p, const D
           }
         }
       }
+      bool odd = false;  // a value scale that 0 x P would not take out, in front of a window or of a later token
       if (masked) {
 #pragma unroll
         for (int u = 0; u < C::RUNS; ++u)
@@ -449,6 +450,7 @@ __device__ __forceinline__ bool decode128_segment(const DecodeParams& p, const D
           for (int h = 0; h < 2; ++h) {
             const int key = key0 + 16 * u + kap + 2 * h;
             if (key >= n) vs[u][h] = 0.f;  // any bits, NaN too
+            odd = odd || !(fabsf(vs[u][h]) < INFINITY);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const int4 l = lim[nt * 4 + t4];  // first and last key of row 2 t, then of row 2 t + 1
@@ -459,7 +461,7 @@ __device__ __forceinline__ bool decode128_segment(const DecodeParams& p, const D
       }
       // P = 2^s and P x value scale x row factor; the row sums take P before its rounding
       float2 pr[C::RUNS][NT][2], pv[C::RUNS][NT][2];
-      bool slow = !open_all;
+      bool slow = !open_all || odd;
       float2 l[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -502,7 +504,8 @@ __device__ __forceinline__ bool decode128_segment(const DecodeParams& p, const D
               for (int h = 0; h < 2; ++h) {
                 at(pr[u][nt][h]) = fast_exp2(at(s[u][nt][h]) - up);
                 at(l[nt]) += at(pr[u][nt][h]);
-                at(pv[u][nt][h]) = at(pr[u][nt][h]) * vs[u][h];
+                // (a masked key's value scale may be NaN)
+                at(pv[u][nt][h]) = at(s[u][nt][h]) == -INFINITY ? 0.f : at(pr[u][nt][h]) * vs[u][h];
                 pm = fmaxf(pm, at(pv[u][nt][h]));
               }
             pm = column_max(pm);
