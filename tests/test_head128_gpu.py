@@ -348,3 +348,33 @@ def test_nan_in_cells_a_row_does_not_see(device, fmt, splits):
     got = U.decode(cache, qb, [4], [n], table, num_splits=splits)
     assert qo.relerr(got[:3], want[:3]) < TOL
     assert np.isnan(got[3]).all()
+
+
+@pytest.mark.parametrize("fmt", ["int4", "k8v4"])
+@pytest.mark.parametrize("drop", [20, 30])
+@pytest.mark.parametrize("back", [False, True])
+def test_values_shrink_while_scores_rise(device, fmt, drop, back):
+    """The first keys hold values 2^drop times those of the later ones, whose scores pass them by about 80 (base 2): what
+    the row is worth lies in the small values, which have to keep their digits (and, with `back`, in the large ones
+    that come again at the end). The rows: one the scores rise for, one they fall for, one they rise half as far, a
+    stranger."""
+    n, lead, nq = 3000, 256, 4
+    rng = np.random.default_rng(50)
+    k0 = rng.standard_normal(HS).astype(np.float32)
+    rise = np.where(np.arange(n) < lead, 0.01, rng.uniform(4.9, 5.0, n)).astype(np.float32)
+    size = np.where(np.arange(n) < lead, 2.0 ** (drop - 20), 2.0 ** -20).astype(np.float32)
+    if back:
+        size[-40:] = size[0]
+    kb = qo.from_f32(rise[:, None, None] * k0[None, None], "bf16")
+    vb = qo.from_f32(size[:, None, None] * rng.standard_normal((n, 1, HS)).astype(np.float32), "bf16")
+    table, nblocks = U.block_tables([n], 16, seed=51)
+    cache = U.Cache(fmt, nblocks, 16, device, nkv=1, hs=HS)
+    pos = np.arange(n)
+    cache.store(kb, vb, table[0].astype(np.int64)[pos // 16] * 16 + pos % 16)
+    qb = qo.from_f32(np.stack([k0, -k0, 0.5 * k0, rng.standard_normal(HS).astype(np.float32)])[None], "bf16")
+    want = U.reference(cache.host_bytes(), cache.layout, qb, [1], [n], table)
+    for splits in (1, 3):
+        got = U.decode(cache, qb, [1], [n], table, num_splits=splits)
+        for h in range(nq):     # each row by itself: their norms differ by 2^drop
+            err = qo.relerr(got[:, h], want[:, h])
+            assert err < TOL, f"row {h}, {splits} splits: relative error {err:.3e}"

@@ -509,11 +509,23 @@ __device__ __forceinline__ bool decode128_segment(const DecodeParams& p, const D
                 pm = fmaxf(pm, at(pv[u][nt][h]));
               }
             pm = column_max(pm);
+            // Where the maximum has moved up, what is left of the output and the products of these keys may be far below
+            // 1 (value scales that fell while the scores rose), where fp16 has no digits for what comes: the factor
+            // is raised, by as much as leaves the largest output (2^20 o: up to 15, a code, times the sum over the
+            // keys) below 2^9, so that keys like the old ones stay within D1_P_LIMIT.
+            float om = fmaxf(z[nt][e], z[nt][e + 2]);
+#pragma unroll
+            for (int ti = 0; ti < 8; ++ti) om = fmaxf(om, fmaxf(o[nt][ti][e], o[nt][ti][e + 2]));
+            const float most = fmaxf(pm * at(F[nt]), column_max(om) * sc * 0x1p11f);
             at(of) = sc;
             if (pm > 0.f && (opening || pm * at(F[nt]) > D1_P_LIMIT)) {
               const float fn = pow2_below_inverse(pm);
               at(of) = sc * (fn / at(F[nt]));
               at(F[nt]) = fn;
+            } else if (most > 0.f && most < 0.015625f) {
+              const float raise = fminf(pow2_below_inverse(most), 0x1p126f / at(F[nt]));
+              at(of) = sc * raise;
+              at(F[nt]) *= raise;
             }
 #pragma unroll
             for (int u = 0; u < C::RUNS; ++u)
