@@ -378,3 +378,26 @@ def test_values_shrink_while_scores_rise(device, fmt, drop, back):
         for h in range(nq):     # each row by itself: their norms differ by 2^drop
             err = qo.relerr(got[:, h], want[:, h])
             assert err < TOL, f"row {h}, {splits} splits: relative error {err:.3e}"
+
+
+@pytest.mark.parametrize("splits", [1, 5, 40])
+def test_nan_query_row_and_its_lse(device, splits):
+    """A row of NaN stays one, its log-sum-exp too (-inf says that a row sees no key); the other rows are untouched."""
+    lens, qlens, nq = [3000], [2], 16
+    cache, table = setup(device, "int4", lens, seed=56)
+    qb = U.make_queries(qlens, seed=57, nq=nq, hs=HS)
+    want, want_lse = U.reference(cache.host_bytes(), cache.layout, qb, qlens, lens, table), \
+        oracle_lse(cache, table, qb, qlens, lens)
+    kc, vc, ks, vs = cache.views
+    q = U.to_torch(qb, device)
+    q[1, 3] = float("nan")
+    out, lse = torch.empty_like(q), torch.empty((2, nq), dtype=torch.float32, device=device)
+    ops.paged_decode(q, kc, vc, out, cu_seqlens_q=torch.tensor([0, 2], dtype=torch.int32, device=device),
+                     max_seqlen_q=2, seqused_k=torch.tensor(lens, dtype=torch.int32, device=device),
+                     max_seqlen_k=lens[0], softmax_scale=HS ** -0.5, block_table=torch.from_numpy(table).to(device),
+                     k_scale_cache=ks, v_scale_cache=vs, num_splits=splits, lse_out=lse)
+    rest = np.ones((2, nq), bool)
+    rest[1, 3] = False
+    got, lse = out.float().cpu().numpy(), lse.cpu().numpy()
+    assert np.isnan(got[1, 3]).all() and np.isnan(lse[1, 3])
+    assert qo.relerr(got[rest], want[rest]) < TOL and np.abs(lse - want_lse)[rest].max() < LSE_TOL

@@ -857,7 +857,7 @@ __global__ void __launch_bounds__(32 * MG_WARPS) merge128_kernel(const MergePara
     }
   }
   if (sink != -INFINITY) T += exp2f(sink - M);  // in the denominator only
-  if (lane == 0 && p.lse_out) p.lse_out[tok * p.lo_t + qh * p.lo_h] = T > 0.f ? M + log2f(T) : -INFINITY;
+  if (lane == 0 && p.lse_out) p.lse_out[tok * p.lo_t + qh * p.lo_h] = T == 0.f ? -INFINITY : M + log2f(T);  // NaN stays
   const float inv = T == 0.f ? 0.f : 1.f / T;
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] *= inv;
