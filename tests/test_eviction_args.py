@@ -215,3 +215,42 @@ def test_lse_output_argument_checks(calls):
     with pytest.raises(ValueError, match="lse_out"):
         ops.paged_decode(q, kc, vc, torch.empty_like(q), lse_out=lse, partials_only=True, **a)
     assert len(calls) == 1
+
+
+def decode_args(**over):
+    """paged_decode of two sequences over a cache of head 128."""
+    kc, vc, ks, vs = cache_views()
+    q = torch.zeros((3, 4, 128), dtype=torch.bfloat16)
+    a = dict(q=q, key_cache=kc, value_cache=vc, out=torch.empty_like(q),
+             cu_seqlens_q=torch.tensor([0, 1, 3], dtype=torch.int32), max_seqlen_q=2,
+             seqused_k=torch.tensor([5, 9], dtype=torch.int32), max_seqlen_k=9, softmax_scale=0.1,
+             block_table=torch.zeros((2, 1), dtype=torch.int32), k_scale_cache=ks, v_scale_cache=vs, num_splits=1)
+    a.update(over)
+    return a
+
+
+def test_decode_takes_a_table_of_one_dimension(calls):
+    """One request's block table as a row, without the sequence axis; for several requests it is refused."""
+    table = torch.arange(4, dtype=torch.int32)
+    one = dict(q=torch.zeros((1, 4, 128), dtype=torch.bfloat16), out=torch.zeros((1, 4, 128), dtype=torch.bfloat16),
+               cu_seqlens_q=torch.tensor([0, 1], dtype=torch.int32), seqused_k=torch.tensor([5], dtype=torch.int32))
+    ops.paged_decode(**decode_args(block_table=table, **one))
+    ops.paged_decode(**decode_args(block_table=table[None], **one))
+    (name, flat), (_, rows) = calls
+    assert name == "qp_paged_decode" and table.data_ptr() in flat and len(flat) == len(_lib.SIGNATURES[name][1])
+    at = flat.index(table.data_ptr())
+    assert flat[at + 1] == 1 and rows[at + 1] == 4     # the row stride, which one sequence does not use
+    with pytest.raises(ValueError, match="block_table"):
+        ops.paged_decode(**decode_args(block_table=table))
+    assert len(calls) == 2
+
+
+@pytest.mark.parametrize("name", ["cu_seqlens_q", "seqused_k", "block_table"])
+def test_decode_names_the_wrong_index_tensor(calls, name):
+    a = decode_args()
+    with pytest.raises(TypeError, match=f"^{name} "):
+        ops.paged_decode(**dict(a, **{name: a[name].long()}))
+    wide = torch.zeros((*a[name].shape[:-1], 2 * 3), dtype=torch.int32)[..., ::2]
+    with pytest.raises(ValueError, match=f"^{name} "):
+        ops.paged_decode(**dict(a, **{name: wide}))
+    assert not calls

@@ -242,7 +242,7 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
                  softcap=0.0, sinks=None, lse_out=None):
     """Split-KV decode of up to 32 query rows per KV head (4 MTP tokens x 6 heads) over the paged cache.
 
-    q / out (tokens, query heads, hs). When `out_fp32_lse` is a tensor (tokens, query heads) fp32, `out` must be fp32
+    q / out (tokens, query heads, hs); block_table (sequences, pages), or a single sequence's row. When `out_fp32_lse` is a tensor (tokens, query heads) fp32, `out` must be fp32
     and receives the RHT-domain output with its base-2 log-sum-exp in `out_fp32_lse` (the partial a sequence-parallel
     rank exchanges); otherwise `out` gets the model-domain output in q's dtype. partials_only=True launches the split
     kernel alone and leaves its partials in the workspace (returned). tokens_after_keys: sequence tokens that follow
@@ -256,7 +256,6 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
     tokens, nq, hs = q.shape
     q_st, q_sh, q_sc = q.stride()
     out_st, out_sh, out_sc = out.stride()
-    bt_st, bt_sc = block_table.stride()
     device = q.device
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
     nkv = lay.nkv
@@ -273,11 +272,12 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
     wbytes = _memo("qp_decode_workspace_bytes", tokens, nq, hs, int(num_splits))
     if ws is None:
         ws = workspace(device, wbytes)
-    int32 = torch.int32
-    if cu_seqlens_q.dtype != int32 or seqused_k.dtype != int32 or block_table.dtype != int32:
-        raise TypeError("cu_seqlens_q, seqused_k and block_table must be int32")
-    if cu_seqlens_q.stride(0) != 1 or seqused_k.stride(0) != 1 or bt_sc != 1:
-        raise ValueError("cu_seqlens_q, seqused_k and block_table rows must be contiguous")
+    int32, bt_st = torch.int32, block_table.stride()
+    if (cu_seqlens_q.dtype != int32 or seqused_k.dtype != int32 or block_table.dtype != int32
+            or cu_seqlens_q.stride(0) != 1 or seqused_k.stride(0) != 1 or bt_st[-1] != 1):
+        _check_index(cu_seqlens_q=cu_seqlens_q, seqused_k=seqused_k, block_table=block_table)   # names the one
+    if len(bt_st) == 1 and num_seqs > 1:
+        raise ValueError(f"a one-dimensional block_table serves one sequence, not {num_seqs}")
     if q_sc != 1 or out_sc != 1:
         raise ValueError("q / out rows must be contiguous")
     dt = _dtype_code(q, "paged_decode")
@@ -296,7 +296,7 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
     if lse_out is not None:
         lse_ptr = _lse_ptr(lse_out, tokens, nq, mode, out_fp32_lse)
     _lib.call("qp_paged_decode", lay.fmt, dt, q.data_ptr(), q_st, q_sh, out.data_ptr(), out_st, out_sh, tokens,
-              num_seqs, cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q), block_table.data_ptr(), bt_st,
+              num_seqs, cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), int(max_seqlen_q), block_table.data_ptr(), bt_st[0],
               *lay.args(), nq, nkv, hs, float(softmax_scale), rht.device_sign_bits(hs, device).data_ptr(),
               int(bool(q_rotated)), int(tokens_after_keys), int(sliding_window), float(softcap or 0.0),
               _sinks_ptr(sinks, nq, mode), mode, lse_ptr, int(num_splits), ws.data_ptr(), ws.nbytes, _stream(device))
