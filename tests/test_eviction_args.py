@@ -254,3 +254,78 @@ def test_decode_names_the_wrong_index_tensor(calls, name):
     with pytest.raises(ValueError, match=f"^{name} "):
         ops.paged_decode(**dict(a, **{name: wide}))
     assert not calls
+
+
+# ---------------------------------------------------------------- tensors on another device
+
+
+class On:
+    """A tensor on a device, as far as the check looks."""
+
+    def __init__(self, index):
+        self.device = torch.device("cuda", index) if index >= 0 else torch.device("cpu")
+
+    def get_device(self):
+        return -1 if self.device.index is None else self.device.index
+
+
+def test_device_check(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    here = torch.device("cuda", 1)
+    ops._check_device(here, out=On(1), lse_out=None)
+    for wrong in (On(0), On(-1)):
+        with pytest.raises(ValueError, match="lse_out"):
+            ops._check_device(here, out=On(1), lse_out=wrong)
+    for elsewhere in (torch.device("cuda", 0), torch.device("cpu")):
+        with pytest.raises(ValueError, match="current device"):
+            ops._check_device(elsewhere, out=On(1))
+
+
+@pytest.mark.parametrize("hs", [128, 256])
+def test_every_tensor_a_kernel_gets_is_checked(calls, monkeypatch, hs):
+    """Each tensor whose address goes to a launch goes through the device check first, at every head size."""
+    seen = {}
+    monkeypatch.setattr(ops, "_check_device", lambda device, **t: seen.update(
+        {id(x): device for x in t.values() if x is not None}))
+    kc, vc, ks, vs = cache_views(hs=hs)
+    q, out = (torch.zeros((3, 4, hs), dtype=torch.bfloat16) for _ in range(2))
+    cu, used = torch.tensor([0, 1, 3], dtype=torch.int32), torch.tensor([5, 9], dtype=torch.int32)
+    table, lse, sinks = torch.zeros((2, 1), dtype=torch.int32), torch.zeros((3, 4)), torch.zeros(4)
+    ws, out32 = torch.empty(64, dtype=torch.uint8), torch.zeros((3, 4, hs))
+    weights = ops.new_attention_weights(ks)
+    common = dict(softmax_scale=0.1, k_scale_cache=ks, v_scale_cache=vs, ws=ws)
+    index = dict(cu_seqlens_q=cu, seqused_k=used, max_seqlen_k=9, block_table=table)
+    monkeypatch.setattr(ops._lib, "load", lambda: type("L", (), {
+        "qp_prefill_workspace_bytes": lambda *a: 0, "qp_prefill_varlen_workspace_bytes": lambda *a: 0})())
+    for fn, given, kw in [
+            (ops.paged_decode, [out, lse, sinks], dict(max_seqlen_q=2, sinks=sinks, lse_out=lse, num_splits=1, **index)),
+            (ops.paged_decode, [out32, lse], dict(max_seqlen_q=2, out_fp32_lse=lse, num_splits=1, **index)),
+            (ops.prefill_varlen, [out, lse, sinks], dict(sinks=sinks, lse_out=lse, **index)),
+            (ops.prefill_varlen, [out32, lse], dict(out_fp32_lse=lse, **index)),
+            (ops.prefill, [out, lse], dict(block_row=table[0], n=9, lse_out=lse)),
+            (ops.prefill, [out32, lse], dict(block_row=table[0], n=9, out_fp32_lse=lse))]:
+        seen.clear()
+        fn(q, kc, vc, given[0], **kw, **common)
+        wanted = given + [kc, ws] + [t for t in kw.values() if isinstance(t, torch.Tensor)]
+        assert all(id(t) in seen for t in wanted), fn.__name__
+        assert set(seen.values()) == {q.device}
+    seen.clear()
+    ops.accumulate_attention_weights(q, kc, vc, weights, lse=lse, max_seqlen_q=2, **index, **common)
+    assert all(id(t) in seen for t in (kc, weights, lse, cu, used, table, ws))
+    seen.clear()
+    ops.evict_cache(kc, vc, weights, seqused_k=used, max_seqlen_k=9, block_table=table, out_block_table=table.clone(),
+                    keep=5, k_scale_cache=ks, v_scale_cache=vs, ws=ws)
+    assert all(id(t) in seen for t in (weights, used, table, ws))
+
+
+@pytest.mark.parametrize("hs", [128, 256, 512])
+def test_host_tensors_are_refused(monkeypatch, hs):
+    """Nothing on the host reaches a launch."""
+    monkeypatch.setattr(ops._lib, "call", lambda *a: pytest.fail("a launch"))
+    kc, vc, ks, vs = cache_views(hs=hs)
+    q = torch.zeros((3, 4, hs), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="cpu"):
+        ops.paged_decode(q, kc, vc, torch.empty_like(q), cu_seqlens_q=torch.tensor([0, 1, 3], dtype=torch.int32),
+                         max_seqlen_q=2, seqused_k=torch.tensor([5, 9], dtype=torch.int32), max_seqlen_k=9,
+                         softmax_scale=0.1, block_table=torch.zeros((2, 1), dtype=torch.int32), k_scale_cache=ks,
+                         v_scale_cache=vs, num_splits=1, ws=torch.empty(64, dtype=torch.uint8))

@@ -53,6 +53,19 @@ def _lse_ptr(lse_out, rows, nq, mode, out_fp32_lse):
     return lse_out.data_ptr()
 
 
+def _check_device(device, **tensors):
+    """The launch goes to the current device: every tensor given has to live there (a kernel that is handed another
+    device's address, or the host's, faults)."""
+    index = device.index
+    if index is None:
+        raise ValueError(f"the tensors are on {device}, the kernels run on the current device, a GPU")
+    if index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {device}, the current device is {torch.cuda.current_device()}")
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
 def _dtype_code(t, what):
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -242,10 +255,11 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
                  softcap=0.0, sinks=None, lse_out=None):
     """Split-KV decode of up to 32 query rows per KV head (4 MTP tokens x 6 heads) over the paged cache.
 
-    q / out (tokens, query heads, hs); block_table (sequences, pages), or a single sequence's row. When `out_fp32_lse` is a tensor (tokens, query heads) fp32, `out` must be fp32
-    and receives the RHT-domain output with its base-2 log-sum-exp in `out_fp32_lse` (the partial a sequence-parallel
-    rank exchanges); otherwise `out` gets the model-domain output in q's dtype. partials_only=True launches the split
-    kernel alone and leaves its partials in the workspace (returned). tokens_after_keys: sequence tokens that follow
+    q / out (tokens, query heads, hs); block_table (sequences, pages), or a single sequence's row. When `out_fp32_lse`
+    is a tensor (tokens, query heads) fp32, `out` must be fp32 and receives the RHT-domain output with its base-2
+    log-sum-exp in `out_fp32_lse` (the partial a sequence-parallel rank exchanges); otherwise `out` gets the
+    model-domain output in q's dtype. partials_only=True launches the split kernel alone and leaves its partials in the
+    workspace (returned). tokens_after_keys: sequence tokens that follow
     the cached keys given here (a sequence-parallel rank holding an earlier range): query token i of a sequence sees
     key k iff k <= seqused_k - qlen + i + tokens_after_keys. sliding_window: vLLM's SLIDING_WINDOW (1 +
     window_size[0], 0 = none): that token then sees only the keys k > its last key - sliding_window. softcap > 0:
@@ -260,8 +274,8 @@ def paged_decode(q, key_cache, value_cache, out, *, cu_seqlens_q, max_seqlen_q, 
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
     nkv = lay.nkv
     num_seqs = cu_seqlens_q.shape[0] - 1
-    if hs == 128:
-        _check_device(device, key_cache=key_cache, out=out)
+    _check_device(device, key_cache=key_cache, out=out, cu_seqlens_q=cu_seqlens_q, seqused_k=seqused_k,
+                  block_table=block_table, sinks=sinks, lse_out=lse_out, out_fp32_lse=out_fp32_lse, ws=ws)
     if num_splits is None:
         keys = window_keys(max_seqlen_k, sliding_window, max_seqlen_q)
         if hs == 128:
@@ -358,6 +372,8 @@ def prefill(q, key_cache, value_cache, out, *, block_row, n, softmax_scale, k_sc
     if q.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("q / out rows must be contiguous")
     dt = _dtype_code(q, "prefill")
+    _check_device(q.device, key_cache=key_cache, out=out, block_row=block_row, lse_out=lse_out,
+                  out_fp32_lse=out_fp32_lse, ws=ws)
     wbytes = _lib.load().qp_prefill_workspace_bytes(qlen, int(n), nq, lay.nkv, hs, int(tokens_after_keys))
     if ws is None:
         ws = workspace(q.device, wbytes)
@@ -394,6 +410,8 @@ def prefill_varlen(q, key_cache, value_cache, out, *, cu_seqlens_q, seqused_k, m
     if q.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("q / out rows must be contiguous")
     dt = _dtype_code(q, "prefill_varlen")
+    _check_device(q.device, key_cache=key_cache, out=out, cu_seqlens_q=cu_seqlens_q, seqused_k=seqused_k,
+                  block_table=block_table, sinks=sinks, lse_out=lse_out, out_fp32_lse=out_fp32_lse, ws=ws)
     chunks = seqused_k.shape[0]
     lib = _lib.load()
     max_k = window_keys(max_seqlen_k, sliding_window, VARLEN_MAX_Q)
@@ -426,16 +444,6 @@ def new_attention_weights(k_scale_cache):
     page's weights of a KV head contiguous."""
     nblocks, block_size, nkv = k_scale_cache.shape
     return torch.zeros((nblocks, nkv, block_size), dtype=torch.float32, device=k_scale_cache.device).transpose(1, 2)
-
-
-def _check_device(device, **tensors):
-    """The launch goes to the current device: every tensor has to live there."""
-    index = device.index
-    if index != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on {device}, the current device is {torch.cuda.current_device()}")
-    for name, t in tensors.items():
-        if t.get_device() != index:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def _check_weights(weights, lay):
@@ -474,7 +482,7 @@ def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_
         raise ValueError(f"lse must be contiguous fp32 ({tokens}, {nq})")
     dt = _dtype_code(q, "accumulate_attention_weights")
     _check_device(q.device, key_cache=key_cache, weights=weights, lse=lse, cu_seqlens_q=cu_seqlens_q,
-                  seqused_k=seqused_k, block_table=block_table)
+                  seqused_k=seqused_k, block_table=block_table, ws=ws)
     num_seqs = cu_seqlens_q.shape[0] - 1
     if ws is None:
         ws = workspace(q.device, _memo("qp_attn_weights_workspace_bytes", tokens, num_seqs, int(max_seqlen_q), nq,
@@ -516,7 +524,7 @@ def evict_cache(key_cache, value_cache, weights, *, seqused_k, max_seqlen_k, blo
     elif seqused_out.dtype != torch.int32 or seqused_out.shape != seqused_k.shape or not seqused_out.is_contiguous():
         raise ValueError("seqused_out must be contiguous int32, one length per sequence")
     _check_device(key_cache.device, weights=weights, seqused_k=seqused_k, block_table=block_table,
-                  seqused_out=seqused_out, **({} if out_block_table is None else {"out_block_table": out_block_table}))
+                  seqused_out=seqused_out, out_block_table=out_block_table, ws=ws)
     kept = torch.empty((num_seqs, lay.nkv, max(keep, 0)), dtype=torch.int32, device=key_cache.device)
     if ws is None:
         ws = workspace(key_cache.device, _memo("qp_evict_workspace_bytes", num_seqs, lay.nkv, int(max_seqlen_k), keep))
