@@ -329,3 +329,42 @@ def test_host_tensors_are_refused(monkeypatch, hs):
                          max_seqlen_q=2, seqused_k=torch.tensor([5, 9], dtype=torch.int32), max_seqlen_k=9,
                          softmax_scale=0.1, block_table=torch.zeros((2, 1), dtype=torch.int32), k_scale_cache=ks,
                          v_scale_cache=vs, num_splits=1, ws=torch.empty(64, dtype=torch.uint8))
+
+
+# ---------------------------------------------------------------- tables and lengths that are too short
+
+
+@pytest.mark.parametrize("over,words", [
+    (dict(max_seqlen_k=17), "block_table"),                                                # two pages, one in the table
+    (dict(block_table=torch.zeros((1, 1), dtype=torch.int32)), "block_table"),             # a row short
+    (dict(seqused_k=torch.tensor([5], dtype=torch.int32)), "seqused_k"),                   # a length short
+    (dict(block_table=torch.zeros(4, dtype=torch.int32)), "block_table"),                  # one row for two sequences
+])
+def test_weights_refuse_short_tables(calls, over, words):
+    with pytest.raises(ValueError, match=words):
+        ops.accumulate_attention_weights(**weights_args(**over))
+    assert not calls
+
+
+@pytest.mark.parametrize("over", [
+    dict(max_seqlen_k=49),                                                                 # four pages, three in the table
+    dict(block_table=torch.zeros((2, 2), dtype=torch.int32)),
+    dict(block_table=torch.zeros(6, dtype=torch.int32)),
+])
+def test_evict_refuses_short_tables(calls, over):
+    """In place a table row is written through as far as the lengths and the budget go."""
+    with pytest.raises(ValueError, match="^block_table"):
+        ops.evict_cache(**evict_args(**over))
+    assert not calls
+
+
+def test_tables_that_just_fit(calls):
+    ops.accumulate_attention_weights(**weights_args(max_seqlen_k=16))
+    ops.evict_cache(**evict_args(max_seqlen_k=48))
+    one = dict(seqused_k=torch.tensor([40], dtype=torch.int32), block_table=torch.zeros(3, dtype=torch.int32))
+    ops.evict_cache(**evict_args(**one))                          # one sequence's row
+    ops.evict_cache(**evict_args(out_block_table=torch.zeros(2, dtype=torch.int32), **one))
+    ops.evict_cache(**evict_args(out_block_table=torch.zeros((2, 2), dtype=torch.int32)))   # 20 of 40 tokens stay
+    with pytest.raises(ValueError, match="^out_block_table"):
+        ops.evict_cache(**evict_args(out_block_table=torch.zeros(1, dtype=torch.int32), **one))
+    assert len(calls) == 5

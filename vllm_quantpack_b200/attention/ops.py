@@ -460,6 +460,14 @@ def _check_index(**tensors):
             raise ValueError(f"{name} rows must be contiguous")
 
 
+def _check_table(name, table, num_seqs, tokens, block_size):
+    """A row of pages for every sequence, wide enough for `tokens` (one sequence's may come without the sequence axis)."""
+    rows = table.shape[0] if table.dim() > 1 else 1
+    if num_seqs > 0 and (rows < num_seqs or table.shape[-1] * block_size < tokens):
+        raise ValueError(f"{name} {tuple(table.shape)} needs pages of {block_size} for {tokens} tokens of each of "
+                         f"{num_seqs} sequences")
+
+
 def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_seqlens_q, max_seqlen_q, seqused_k,
                                  max_seqlen_k, softmax_scale, block_table, k_scale_cache, v_scale_cache,
                                  q_rotated=False, ws=None, tokens_after_keys=0, sliding_window=0, softcap=0.0):
@@ -469,7 +477,8 @@ def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_
     `lse_out`. Summed over the query tokens (one, or a whole prompt) and the query heads of each KV head. The call's own
     tokens have no earlier weight: theirs is stored, so pages need no clearing before reuse as long as every token
     enters through such a call; a first call that covers only the last tokens of a prompt wants the other cells zeroed.
-    Cells past a sequence's length are left as they are. Calls that overlap on the GPU (two streams, two graphs replayed
+    Cells past a sequence's length are left as they are. max_seqlen_k bounds the lengths, and block_table has pages for as
+    many tokens. Calls that overlap on the GPU (two streams, two graphs replayed
     at once) need workspaces of their own (`ws`). Returns `weights`."""
     tokens, nq, hs = q.shape
     q_st, q_sh, q_sc = q.stride()
@@ -484,6 +493,9 @@ def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_
     _check_device(q.device, key_cache=key_cache, weights=weights, lse=lse, cu_seqlens_q=cu_seqlens_q,
                   seqused_k=seqused_k, block_table=block_table, ws=ws)
     num_seqs = cu_seqlens_q.shape[0] - 1
+    if seqused_k.shape[0] < num_seqs:
+        raise ValueError(f"seqused_k has {seqused_k.shape[0]} lengths for {num_seqs} sequences")
+    _check_table("block_table", block_table, num_seqs, int(max_seqlen_k), lay.block_size)
     if ws is None:
         ws = workspace(q.device, _memo("qp_attn_weights_workspace_bytes", tokens, num_seqs, int(max_seqlen_q), nq,
                                        lay.nkv, hs))
@@ -505,6 +517,7 @@ def evict_cache(key_cache, value_cache, weights, *, seqused_k, max_seqlen_k, blo
     hold the pages), or with `out_block_table` (int32 (seqs, pages)) into other pages, the old ones left as they are: a
     sequence whose pages others share (a common prompt). Returns (kept, seqused): the old positions (seqs, KV heads,
     keep) int32, -1 behind the last, and the new lengths (`seqused_out` if given, which may be `seqused_k` itself).
+    max_seqlen_k bounds the lengths, and block_table has pages for as many tokens.
     Calls that overlap on the GPU need workspaces of their own (`ws`)."""
     int4 = key_cache.dtype == torch.uint8
     hs = (key_cache.shape[-1] - 4) * 2 if int4 else key_cache.shape[-1]
@@ -512,13 +525,10 @@ def evict_cache(key_cache, value_cache, weights, *, seqused_k, max_seqlen_k, blo
     _check_weights(weights, lay)
     _check_index(seqused_k=seqused_k, block_table=block_table)
     num_seqs, keep = seqused_k.shape[0], int(keep)
-    if block_table.shape[0] < num_seqs:
-        raise ValueError("block_table needs a row for every sequence")
+    _check_table("block_table", block_table, num_seqs, int(max_seqlen_k), lay.block_size)
     if out_block_table is not None:
         _check_index(out_block_table=out_block_table)
-        if out_block_table.shape[0] < num_seqs or out_block_table.shape[1] * lay.block_size < min(keep,
-                                                                                                   int(max_seqlen_k)):
-            raise ValueError("out_block_table needs pages for every sequence's kept tokens")
+        _check_table("out_block_table", out_block_table, num_seqs, min(keep, int(max_seqlen_k)), lay.block_size)
     if seqused_out is None:
         seqused_out = torch.empty_like(seqused_k)
     elif seqused_out.dtype != torch.int32 or seqused_out.shape != seqused_k.shape or not seqused_out.is_contiguous():
