@@ -368,3 +368,45 @@ def test_tables_that_just_fit(calls):
     with pytest.raises(ValueError, match="^out_block_table"):
         ops.evict_cache(**evict_args(out_block_table=torch.zeros(1, dtype=torch.int32), **one))
     assert len(calls) == 5
+
+
+# ---------------------------------------------------------------- workspaces
+
+
+def test_workspaces_of_streams(monkeypatch):
+    """Eager calls on two streams get two buffers; captured ones, and those on the default stream, the device's own."""
+    monkeypatch.setattr(ops, "_workspaces", {})
+    monkeypatch.setattr(ops, "_retired", [])
+    now = dict(stream=0, capturing=False)
+    monkeypatch.setattr(ops, "_stream", lambda device: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+
+    def get(stream, nbytes=100, capturing=False):
+        now.update(stream=stream, capturing=capturing)
+        return ops.workspace("cpu", nbytes)
+
+    own = get(0)
+    a, b = get(7), get(9)
+    assert len({t.data_ptr() for t in (own, a, b)}) == 3
+    assert get(7) is a and get(9) is b and get(0) is own
+    assert get(7, capturing=True) is own and get(11, capturing=True) is own
+    now.update(stream=7, capturing=False)
+    big = ops.reserve_workspace("cpu", 3 << 20)        # grown for a capture to come, from whatever stream
+    assert big.numel() >= 3 << 20 and get(13, 3 << 20, capturing=True) is big and get(0) is big
+    assert get(7) is a
+    assert any(t is own for t in ops._retired)         # a graph may hold the smaller one
+
+
+def test_workspace_reserved_at_start(monkeypatch):
+    """The metadata builder's reservation covers captured steps and eager ones on its stream."""
+    from vllm_quantpack_b200.attention import int4_kv
+    seen = []
+    monkeypatch.setattr(ops, "reserve_workspace", lambda device, n: seen.append(("own", device, n)))
+    monkeypatch.setattr(ops, "workspace", lambda device, n: seen.append(("stream", device, n)))
+    monkeypatch.setattr(ops, "sm_count", lambda device: 148)
+    monkeypatch.setattr(int4_kv, "decode_workspace_bound", lambda *a: 12345)
+    model = type("M", (), dict(get_num_attention_heads=lambda s, p: 24, get_num_kv_heads=lambda s, p: 4,
+                               get_head_size=lambda s: 256, max_model_len=4096))()
+    config = type("C", (), dict(model_config=model, parallel_config=None))()
+    int4_kv.reserve_decode_workspace(type("B", (), dict(seq_threshold_3D=16))(), config, "cuda:0")
+    assert seen == [("own", "cuda:0", 12345), ("stream", "cuda:0", 12345)]

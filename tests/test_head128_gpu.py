@@ -401,3 +401,37 @@ def test_nan_query_row_and_its_lse(device, splits):
     got, lse = out.float().cpu().numpy(), lse.cpu().numpy()
     assert np.isnan(got[1, 3]).all() and np.isnan(lse[1, 3])
     assert qo.relerr(got[rest], want[rest]) < TOL and np.abs(lse - want_lse)[rest].max() < LSE_TOL
+
+
+def test_two_streams_at_once(device):
+    """Decodes and weights of two requests on two streams, each with the default workspace: what one writes there is
+    not the other's."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    runs = []
+    for i, n in enumerate((60000, 45000)):
+        cache, table = setup(device, "int4", [n], seed=60 + i)
+        q = U.to_torch(U.make_queries([2], seed=62 + i, nq=16, hs=HS), device)
+        args = dict(cu_seqlens_q=torch.tensor([0, 2], dtype=torch.int32, device=device), max_seqlen_q=2,
+                    seqused_k=torch.tensor([n], dtype=torch.int32, device=device), max_seqlen_k=n,
+                    softmax_scale=HS ** -0.5, block_table=torch.from_numpy(table).to(device),
+                    k_scale_cache=cache.views[2], v_scale_cache=cache.views[3])
+        runs.append((cache, q, args))
+
+    def step(i):
+        cache, q, args = runs[i]
+        out, lse = torch.empty_like(q), torch.empty((2, 16), dtype=torch.float32, device=device)
+        weights = ops.new_attention_weights(cache.views[2])
+        ops.paged_decode(q, *cache.views[:2], out, lse_out=lse, **args)
+        ops.accumulate_attention_weights(q, *cache.views[:2], weights, lse=lse, **args)
+        return out, lse, weights
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got.append((i, step(i)))
+    torch.cuda.synchronize()
+    for i, tensors in got:
+        assert all(torch.equal(a, b) for a, b in zip(tensors, want[i]))

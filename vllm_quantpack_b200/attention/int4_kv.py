@@ -412,7 +412,9 @@ def reserve_decode_workspace(builder, vllm_config, device):
             head = int(model.get_head_size())
         except Exception:
             head = max(HEAD_SIZES)
-        ops.workspace(device, decode_workspace_bound(rows, nq, nkv, max_len, ops.sm_count(device), head))
+        bound = decode_workspace_bound(rows, nq, nkv, max_len, ops.sm_count(device), head)
+        ops.reserve_workspace(device, bound)   # captured steps
+        ops.workspace(device, bound)           # eager ones on this stream: the same buffer on the default stream
     except Exception:
         pass
 

@@ -19,6 +19,9 @@ MAX_Q_DECODE_ROWS = 32      # query rows (tokens x query heads per KV head) one 
 
 
 def _stream(device):
+    """The current stream's handle (of an indexed device without building the stream object: every op asks twice)."""
+    if type(device) is torch.device and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -191,10 +194,24 @@ _retired = []
 
 
 def workspace(device, nbytes):
-    """A per-device scratch buffer for the split-KV partials, grown geometrically and kept for the process. A
-    buffer that is outgrown stays allocated too: a CUDA graph captured earlier may still hold its address. Growing
-    it inside a CUDA-graph capture allocates from the graph's pool: reserve the largest size before capturing."""
-    key = _device_key(device)
+    """A scratch buffer for the split-KV partials, grown geometrically and kept for the process: the device's own for
+    calls on the default stream and those captured into a graph, one more for every other stream with eager calls (calls
+    on two streams may overlap). A buffer that is outgrown stays allocated too: a CUDA graph captured earlier may still
+    hold its address. Growing it inside a CUDA-graph capture allocates from the graph's pool: reserve the largest size
+    before capturing (`reserve_workspace`)."""
+    stream = _stream(device)
+    if stream and torch.cuda.is_current_stream_capturing():
+        stream = 0
+    return _workspace(_device_key(device), stream, nbytes)
+
+
+def reserve_workspace(device, nbytes):
+    """Grows the device's own buffer, whatever the current stream: what captured calls use."""
+    return _workspace(_device_key(device), 0, nbytes)
+
+
+def _workspace(device, stream, nbytes):
+    key = (device, stream)
     ws = _workspaces.get(key)
     if ws is not None and ws.numel() >= nbytes:  # the common case: no growth, no lock
         return ws
@@ -478,8 +495,8 @@ def accumulate_attention_weights(q, key_cache, value_cache, weights, *, lse, cu_
     tokens have no earlier weight: theirs is stored, so pages need no clearing before reuse as long as every token
     enters through such a call; a first call that covers only the last tokens of a prompt wants the other cells zeroed.
     Cells past a sequence's length are left as they are. max_seqlen_k bounds the lengths, and block_table has pages for as
-    many tokens. Calls that overlap on the GPU (two streams, two graphs replayed
-    at once) need workspaces of their own (`ws`). Returns `weights`."""
+    many tokens. Eager calls on two streams may overlap; graphs that are replayed at once, or beside eager calls on the
+    default stream, need workspaces of their own (`ws`). Returns `weights`."""
     tokens, nq, hs = q.shape
     q_st, q_sh, q_sc = q.stride()
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
@@ -518,7 +535,7 @@ def evict_cache(key_cache, value_cache, weights, *, seqused_k, max_seqlen_k, blo
     sequence whose pages others share (a common prompt). Returns (kept, seqused): the old positions (seqs, KV heads,
     keep) int32, -1 behind the last, and the new lengths (`seqused_out` if given, which may be `seqused_k` itself).
     max_seqlen_k bounds the lengths, and block_table has pages for as many tokens.
-    Calls that overlap on the GPU need workspaces of their own (`ws`)."""
+    Workspaces (`ws`) as for `accumulate_attention_weights`."""
     int4 = key_cache.dtype == torch.uint8
     hs = (key_cache.shape[-1] - 4) * 2 if int4 else key_cache.shape[-1]
     lay = CacheLayout.of(key_cache, value_cache, k_scale_cache, v_scale_cache, hs)
