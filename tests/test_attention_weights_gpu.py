@@ -356,3 +356,15 @@ def test_nan_in_cells_no_row_sees(device, fmt, hs, qlen):
               sliding_window=window).cpu().numpy()
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= rtol * added + 2.0 ** -23 * np.abs(want) + 1e-37).all()
+
+
+@pytest.mark.parametrize("prompt", [1, 150])
+def test_nine_hundred_requests(device, prompt):
+    """More requests than a CTA has threads, with some that have no query or no key among them: the scans that find a
+    CTA's share and a query tile's place go on from one round of threads to the next. Few rows, and with a prompt of
+    several tiles near the end."""
+    rng = np.random.default_rng(45)
+    lens = [int(n) for n in rng.integers(0, 50, 900)]
+    qlens = [min(int(rng.integers(0, 3)), n) if n else int(rng.integers(0, 2)) for n in lens]
+    lens[880], qlens[880] = 700, prompt
+    check(device, "int4", 128, 8, 2, qlens, lens, seed=46)

@@ -202,3 +202,9 @@ def test_two_evictions_in_a_row(device):
         assert np.array_equal(kept.cpu().numpy(), want) and used.tolist() == list(lens)
     assert np.array_equal(cache.phys.cpu().numpy().transpose(0, 2, 1, 3), pages)
     assert np.array_equal(weights.cpu().numpy(), w)
+
+
+def test_more_tokens_than_the_selection_holds(device):
+    """Above 16 x 47,104 tokens a part of the weights does not fit the cluster's shared memory and is read again."""
+    check(device, "int4", 128, 1, [760001], 5000, 4, 100, seed=12)
+    check(device, "int4", 128, 1, [760001, 9], 700000, 0, 0, out=True, make=ties, seed=13)

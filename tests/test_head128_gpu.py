@@ -435,3 +435,29 @@ def test_two_streams_at_once(device):
     torch.cuda.synchronize()
     for i, tensors in got:
         assert all(torch.equal(a, b) for a, b in zip(tensors, want[i]))
+
+
+@pytest.mark.parametrize("tokens", [2, 4])
+def test_nine_hundred_requests(device, tokens):
+    """More requests than a CTA has threads, with some that have no query or no key among them and a long one near the
+    end: the scan that finds a CTA's share goes on from one round of threads to the next."""
+    rng = np.random.default_rng(58)
+    lens = [int(n) for n in rng.integers(0, 60, 900)]
+    qlens = [min(int(rng.integers(0, tokens + 1)), n) if n else int(rng.integers(0, 2)) for n in lens]
+    lens[880], qlens[880], qlens[0], lens[0] = 5000, tokens, tokens, 40
+    cache, table = setup(device, "int4", lens, seed=59, nkv=2)
+    qb = U.make_queries(qlens, seed=60, nq=8, hs=HS)
+    got = U.decode(cache, qb, qlens, lens, table)
+    data, at = cache.host_bytes(), 0
+    rows, want = [], []
+    for i, (ql, n) in enumerate(zip(qlens, lens)):
+        if ql and n:
+            want.append(U.reference(data, cache.layout, qb[at:at + ql], [ql], [n], table[i:i + 1]))
+            rows += range(at, at + ql)
+        elif ql:
+            assert (got[at:at + ql] == 0).all()
+        at += ql
+    want = np.concatenate(want)
+    assert qo.relerr(got[rows], want) < TOL
+    worst = np.linalg.norm(got[rows] - want, axis=-1) / np.linalg.norm(want, axis=-1)
+    assert worst.max() < 4 * TOL    # no row is another's
