@@ -550,6 +550,18 @@ def test_k8v4_call_outside_the_kernels_raises(monkeypatch):
     assert not stock_calls
 
 
+def test_k8v4_refusal_at_head_128_names_the_ops(monkeypatch):
+    """The entry point does not route head 128, the ops serve it: the message says both."""
+    rec = Recorder(monkeypatch)
+    stock, stock_calls = _stock_recorder()
+    fn = int4_kv.make_unified_attention(stock)
+    q, _, out, args = _step([1], [5000], hs=128)
+    kc8 = torch.zeros((4, 16, NKV, 128), dtype=torch.int8)
+    with pytest.raises(NotImplementedError, match=r"not routed.*attention\.ops serve head 128"):
+        fn(q, kc8, kc8, out, **args)
+    assert not stock_calls and not rec.calls
+
+
 def test_step_plan_is_made_once_per_step(monkeypatch):
     """Every layer of a step gets the same length tensors: only the first layer reads them (one host read)."""
     Recorder(monkeypatch)

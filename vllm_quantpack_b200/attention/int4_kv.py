@@ -12,10 +12,11 @@ copy of vLLM's Triton kernel and launcher; this module instead replaces the stoc
   reshape_and_cache_int4   fused RHT + quantize + pack store, int4 and k8v4 (k8v4_kv.py:152-163)
   single_rht               the transform both of the above apply, so any stock path left in use stays consistent
 
-Head sizes 256 and 512 (Gemma 4's global layers, int4_kv.py:302-305) are served. Calls the B200 path does not cover
-(sliding window, softcap, sinks, ALiBi, qq_bias, FP8 output, mm_prefix ranges, another head size) go to the stock
-`unified_attention_int4`, unchanged, for an int4 cache, and raise for a k8v4 cache (no stock kernel reads it). The
-stock `_launch_packed_attn` is left in place: only that stock path reaches it. The same environment switches are honoured:
+Head sizes 256 and 512 (Gemma 4's global layers, int4_kv.py:302-305) are served. Calls this module does not route to
+the B200 kernels (ALiBi, qq_bias, FP8 output, mm_prefix ranges, another head size; `ops` takes head 128 when called) go
+to the stock `unified_attention_int4`, unchanged, for an int4 cache, and raise for a k8v4 cache (no stock kernel reads
+it). The stock `_launch_packed_attn` is left in place: only that stock path reaches it. The same environment switches are
+honoured:
 VLLM_QUANTPACK_INT4_KV=0 (no patch), VLLM_QUANTPACK_INT4_FA_PREFILL=0 (prefill chunks stay stock),
 VLLM_QUANTPACK_INT4_DECODE="tile,warps,segments[,rows]" (segments: split count of the decode, "auto" = per call),
 VLLM_QUANTPACK_INT4_TILES (accepted; the B200 prefill tiles are fixed at 128 x 64).
@@ -32,7 +33,7 @@ PACKED_DTYPES = ("int4_per_token_head", "k8v4_per_token_head")   # caches served
 MAX_Q_SPLIT_KV = 4               # MTP / EAGLE verification with up to 3 draft tokens
 MAX_DECODE_ROWS = 32             # query tokens x query heads per KV head one decode CTA holds
 LONG_ROWS = 2048                 # query rows (tokens x heads per KV head) that make a chunk long at any context
-HEAD_SIZES = (256, 512)          # head sizes of the attention kernels
+HEAD_SIZES = (256, 512)          # head sizes this module routes to the B200 kernels (the ops serve 128 too)
 PREFILL_TILES_DEFAULT = (128, 64, 10, 1)   # (BLOCK_M, TILE, warps, CTAs per SM) of the tcgen05 prefill kernel
 DECODE_TILES_DEFAULT = (64, 4, "auto")
 DECODE_MAX_M = 32
@@ -214,8 +215,8 @@ def make_unified_attention(stock_unified, prefill_on=True):
             if k8v4_kv.is_k8v4(k_cache):
                 raise NotImplementedError(
                     f"{k8v4_kv.NAME}: ALiBi, qq_bias, FP8 output, mm_prefix ranges and head sizes other than "
-                    f"{HEAD_SIZES} are not served by the B200 kernels, and vLLM's stock int4 kernel cannot read a "
-                    f"k8v4 cache")
+                    f"{HEAD_SIZES} are not routed to the B200 kernels (the ops of vllm_quantpack_b200.attention.ops "
+                    f"serve head 128 when called), and vLLM's stock int4 kernel cannot read a k8v4 cache")
             return stock_unified(q, k_cache, v_cache, out, **stock_args())
         group = q.shape[1] // k_cache.shape[2]
         window = sliding_window_of(window_size)
