@@ -228,3 +228,28 @@ def test_mixed_step_through_the_router(device, stock, fmt, softcap, sinks):  # n
     err = qo.relerr(got[sample], np.concatenate(want))
     assert err < TOL, f"{fmt}: relative error {err:.3e}"
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("fmt", ["int4", "k8v4"])
+@pytest.mark.parametrize("nq,nkv,hs", [(24, 4, 256), (16, 2, 512)])
+@pytest.mark.parametrize("qlen", [1, 3])
+def test_nan_in_front_of_the_window(device, fmt, nq, nkv, hs, qlen):
+    """Cells in front of the first token's window hold NaN scales (their pages may be another request's by now): no row
+    sees them, decode and varlen."""
+    n, window = 2101, 300
+    cache, table, qb = build(device, fmt, [qlen], [n], nq=nq, nkv=nkv, hs=hs, seed=90)
+    want = U.reference(cache.host_bytes(), cache.layout, qb, [qlen], [n], table, sliding_window=window)
+    raw = cache.phys.view(torch.uint8)
+    for i in range(n - qlen + 1 - window):
+        raw[int(table[0][i // BS]), :, i % BS] = 0xFF
+    for splits in (None, 1):
+        got = U.decode(cache, qb, [qlen], [n], table, num_splits=splits, sliding_window=window)
+        assert qo.relerr(got, want) < TOL
+    kc, vc, ks, vs = cache.views
+    q = U.to_torch(qb, device)
+    out = torch.empty_like(q)
+    ops.prefill_varlen(q, kc, vc, out, cu_seqlens_q=torch.tensor([0, qlen], dtype=torch.int32, device=device),
+                       seqused_k=torch.tensor([n], dtype=torch.int32, device=device), max_seqlen_k=n,
+                       block_table=torch.from_numpy(table).to(device), softmax_scale=hs ** -0.5, k_scale_cache=ks,
+                       v_scale_cache=vs, sliding_window=window)
+    assert qo.relerr(out.float().cpu().numpy(), want) < TOL

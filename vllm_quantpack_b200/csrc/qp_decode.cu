@@ -494,7 +494,10 @@ __global__ void __maxnreg__((DecWarps<HS, RL>::REGS)) decode_kernel(const Decode
       const uint8_t* cell = smem + SM::OFF_RAW + stage * SM::RAW + (kl - part * SK) * CELL;
       const uint32_t kw = *reinterpret_cast<const uint32_t*>(cell + CL::KS);
       const uint32_t vw = *reinterpret_cast<const uint32_t*>(cell + CL::VS);
-      const bool valid = (tile0 + i) * DEC_TILE + kl < n;
+      // past the sequence, and in front of the first token's window (its page may be another request's by now), a cell
+      // may hold any bits, a NaN value scale too, which P = 0 would not take out
+      const int key = (tile0 + i) * DEC_TILE + kl;
+      const bool valid = key < n && (!FEAT || p.window == 0 || key > vis_base - p.window);
       float ks, kz = 0.f;
       if constexpr (FMT == FMT_INT4) {
         ks = __uint_as_float(kw & 0xFFFFFFF0u);
