@@ -87,8 +87,9 @@ int qp_single_rht(const float* x, float* y, int64_t rows, int head_size, int inv
 int qp_decode_num_splits(int num_seqs, int num_kv_heads, int max_seqlen_k, int sm_count);
 
 /* The same for a head size: 256 and 512 as above; at 128 the most partials a row of a batch gets, where max_rows is
- * max_seqlen_q * (num_q_heads / num_kv_heads) (the batch's tiles are shared evenly over the GPU whatever the lengths,
- * and num_splits bounds the shares that meet in one sequence and KV head). */
+ * max_seqlen_q * (num_q_heads / num_kv_heads) (the batch's tiles are shared evenly over the GPU, by the lengths on the
+ * device; num_splits bounds the shares that meet in one sequence and KV head, so a sequence many times as long as the
+ * others is cut less evenly). */
 int qp_decode_num_splits_head(int head_size, int max_rows, int num_seqs, int num_kv_heads, int max_seqlen_k,
                               int sm_count);
 
@@ -107,7 +108,8 @@ int64_t qp_decode_workspace_bytes(int64_t num_q_tokens, int num_q_heads, int hea
  * sliding_window: vLLM's SLIDING_WINDOW (1 + window_size[0]; 0 = none): query token i whose last visible key is p
  * sees the keys [p - sliding_window + 1, p] only, as the stock kernel masks them (vllm/v1/attention/ops/
  * triton_attention_helpers.py:196-218 and triton_unified_attention.py:533-536, vLLM 0.22); the splits then cover
- * only the tiles of the window, so num_splits should come from min(context, window + max_seqlen_q + 127).
+ * only the tiles of the window, so num_splits should come from min(context, window + max_seqlen_q + 127). Cells behind
+ * seqused_k and in front of the first query token's window may hold any bits (their pages have to exist).
  * softcap: vLLM's logit softcap (0 = none): every score S = softmax_scale / head_size x q.k becomes
  * softcap x tanh(S / softcap) before the softmax (vllm/v1/attention/ops/triton_attention_helpers.py:28-36,
  * triton_unified_attention.py:513-514, vLLM 0.22).
@@ -248,9 +250,12 @@ int64_t qp_attn_weights_workspace_bytes(int64_t num_q_tokens, int num_seqs, int 
  * call of the same rows returned (lse_out), sinks included; a row of lse -inf adds nothing. The tokens of the call
  * itself (keys at n - qlen + tokens_after_keys and on, n = seqused_k) have no earlier weight: theirs is stored, not
  * added. Cells past seqused_k are left as they are. The keys of a page that several sequences of the call share get
- * every sequence's weight, added in no fixed order. cu_seqlens_q, seqused_k, block_table, the cache, softmax_scale,
- * q_rotated, tokens_after_keys, sliding_window and softcap as in qp_paged_decode; max_seqlen_q any length (a whole
- * prompt, or the last chunk of one); max_seqlen_k bounds seqused_k (keys from it on are not visited). Head sizes 128,
+ * every sequence's weight, added in no fixed order. A call's weight of a key is within 1e-5 of its value, whatever the
+ * number of rows (for scores of some tens: 2^-20 of the sum of a score's products' magnitudes comes on top), and enters
+ * the fp32 sum with one rounding a call. cu_seqlens_q, seqused_k, block_table (pages for max_seqlen_k tokens), the
+ * cache, softmax_scale, q_rotated, tokens_after_keys, sliding_window and softcap as in qp_paged_decode; max_seqlen_q any
+ * length (a whole prompt, or the last chunk of one); max_seqlen_k bounds seqused_k (keys from it on are not visited).
+ * Cells in front of every row's window may hold any bits and get nothing. Head sizes 128,
  * 256 and 512. No counterpart in the reference. */
 int qp_accumulate_attn_weights(int fmt, int dtype, const void* q, int64_t q_stride_token, int64_t q_stride_head,
                                int64_t num_q_tokens, int num_seqs, const int32_t* cu_seqlens_q,

@@ -42,8 +42,8 @@ struct DecodeParams {
   // softcap > 0: every score S (natural units) becomes softcap x tanh(S / softcap) before the softmax, vLLM's
   // apply_softcap (vllm/v1/attention/ops/triton_attention_helpers.py:28-36, triton_unified_attention.py:513-514)
   float softcap;
-  // head 128 only: the num_seqs sequences of cu_seqlens_q / seqused_k share the grid's CTAs evenly whatever their
-  // lengths (set by launch_decode128), instead of num_splits equal parts of each
+  // head 128 only: the num_seqs sequences of cu_seqlens_q / seqused_k share the grid's CTAs by their lengths (set by
+  // launch_decode128), each cut into num_splits parts at most, instead of num_splits equal parts of each
   int num_seqs, balanced;
   int num_splits;
   float* part_o;    // [tokens][nq][splits][HS]

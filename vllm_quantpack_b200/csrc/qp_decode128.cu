@@ -150,12 +150,12 @@ __device__ __forceinline__ void close_slots(const DecodeParams& p, const DecodeS
 
 // A balanced launch: the tiles of all (sequence, KV head) pairs in a row, sequence by sequence, head by head, each pair
 // led by C::START units that stand for what starting on it costs a CTA (its query rows, the first copies' latency, the
-// merge of the warps), cut into shares of `share` units; CTA c takes the c-th. Measured (us; START 32 / 64 / 128): 12
-// rows over 131,072 keys 39.0 / 35.0 / 35.4, a ragged k8v4 batch of 16 rows 81.4 / 75.4 / 79.9, 8 rows over 1000 keys
-// 12.4 / 14.4 / 14.4; without it, CTAs that meet two pairs end last (n 131,072: 45). The
+// merge of the warps), cut into shares of `share` units; CTA c takes the c-th. Measured in one sweep (us; START 32 / 64
+// / 128): 12 rows over 131,072 keys 39.0 / 35.0 / 35.4 (now 36), a ragged k8v4 batch of 16 rows 81.4 / 75.4 / 79.9, 8
+// rows over 1000 keys 12.4 / 14.4 / 14.4; without it, CTAs that meet two pairs end last (n 131,072: 45). The
 // shares with tiles of a pair are its partials, in order. share: as even as the grid allows, at least a tile a warp,
 // and so long that no pair meets more than num_splits shares (T <= share (num_splits - 1) tiles meet at most
-// num_splits).
+// num_splits): a request much longer than the others, cut into num_splits shares at most, leaves CTAs without work.
 struct Share {
   int64_t share, hi;  // units of a share, end of this CTA's
   int64_t unit;       // where the pair of (seq, kvh) starts
@@ -307,7 +307,9 @@ __device__ __forceinline__ bool decode128_segment(const DecodeParams& p, const D
   for (int k = 0; k < STAGES - 1; ++k) issue();
 
   // ---- query rows: one warp per row, rotated, scaled by a power of two to |q| < 2^14 and rounded to fp16 in the
-  // operand's order; the rounding (2^-12 of a value) is the size of the model dtype's own
+  // operand's order. The rounding (2^-12 of a value) is what the head 256 / 512 kernel takes too: through the scores it
+  // is 4e-4 of an output (P's to fp16 is 2e-4), below a bf16 output's own rounding (1.6e-3) and twice an fp16 output's
+  // (2.1e-4). A second fp16 term would leave an fp16 output 2.8e-4 off, for a third more time (16 rows: 76 -> 100 us).
   float4* rowp = reinterpret_cast<float4*>(smem + C::OFF_ROW);
   int4* lim = reinterpret_cast<int4*>(smem + C::OFF_LIM);
   for (int r = warp; r < ROWS; r += WARPS) {

@@ -28,8 +28,10 @@
 // full rate); held by the hand-offs between the roles, no one of them alone (without the second term 71 us, without the
 // conversion 68, with an eighth of the copies 62). Many rows (prompts): a group of two key tiles stays in TMEM while all
 // query tiles that see it stream through L2, so a query tile's bytes serve 256 keys; bound by the MMAs of the two terms
-// at head 256 (1024 queries x 40,960 keys, 24 / 4 heads: 0.67 ms, 1,515 TFLOP/s with both terms, 92 % of the library
-// product's peak), by the exponentials and the score reads at head 128 (three whole prompts to 2,777 tokens: 0.28 ms).
+// at head 256 (1024 queries x 40,960 keys, 24 / 4 heads: 0.68 ms at full clocks, 1,500 TFLOP/s with both terms, 91 % of
+// the library product's peak; 0.78 ms, 79 %, when calls follow one another under the power cap). At head 128 no pipe is
+// full (three whole prompts to 2,777 tokens: 0.28 ms, of it 0.19 this kernel and most of the rest K4q; tensor 44 %, XU
+// 44 %): two summing warps a scheduler wait for their score reads.
 // The (key group, query tile) steps of all sequences and KV heads are cut evenly over the CTAs; where a cut falls
 // inside a group its parts go to the workspace and K4f adds them in order, so the sum does not depend on timing.
 #include <limits.h>
